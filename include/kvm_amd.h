@@ -53,7 +53,7 @@
 extern "C" {
 #endif
 
-#define KVM_ABI_VERSION 12
+#define KVM_ABI_VERSION 13
 
 #define KVM_OK 0
 #define KVM_EINVAL (-1)
@@ -382,10 +382,111 @@ int kvm_gemm_small_tile_rows(int64_t M, int64_t N);
 int kvm_gemm_small_packed(const void *x, int64_t x_st, const void *wp, void *y, int64_t y_st, int64_t M,
                           int64_t N, int64_t K, int tile_rows, int epilogue, void *stream);
 
+/* ---- operators on a decoder's logits ---- */
+
+/* Value types of logits (and of a teacher's values). */
+#define KVM_BF16 0
+#define KVM_F16 1
+#define KVM_F32 2
+
+/* Rows of logits: row r = o * inner + i (o < outer, i < inner) starts at
+ * data + o * s_outer + i * s_inner (elements of dtype) and holds vocab
+ * contiguous values.  Any alignment of the type, any vocab in [1, 2^20],
+ * outer * inner in [1, 2^31). */
+typedef struct kvm_logits {
+  const void *data;
+  int64_t dtype; /* KVM_BF16, KVM_F16, KVM_F32 */
+  int64_t vocab;
+  int64_t outer, inner;
+  int64_t s_outer, s_inner;
+} kvm_logits;
+
+/* The k largest logits of every row (1 <= k <= min(vocab, 512)), largest
+ * first, equal ones by rising index: values [rows, k] (the logits' type),
+ * indices [rows, k], and optionally (NULL: not wanted) rest [rows], the
+ * log-sum-exp of x / temperature over all other logits (-infinity where there
+ * are none).  A NaN counts as -infinity.  What a teacher keeps of its logits
+ * for kvm_head_loss. */
+int kvm_top_logits(const kvm_logits *logits, int64_t k, double temperature, void *values, int64_t *indices,
+                   float *rest, void *stream);
+
+/* One token per row, drawn at a temperature from the tokens that top-k, top-p
+ * and min-p keep, with given uniform numbers.
+ * With the row's logits in falling order (equal ones by rising index; a NaN
+ * counts as -infinity), x_0 first, token j has the whole-number weight
+ * w_j = floor(2^42 exp((x_j - x_0) / T) + 1/2); a weight of 0 is never drawn.
+ * top_k (<= 0: off) keeps the first top_k tokens; top_p (>= 1: off) of these
+ * the shortest prefix whose weight reaches top_p times theirs; min_p (<= 0:
+ * off) of these the tokens with w_j >= min_p 2^42.  The first token is always
+ * kept.  With C the weight kept, the token is the first whose running sum
+ * passes floor(u C), and its log-probability (x_j - x_0) / T - ln(C 2^-42).
+ * T <= 0 (or NaN) takes the first token, log-probability 0.  A row of
+ * -infinity (and NaN) gives token 0 and the log-probability NaN.
+ * Each setting is a device array [rows] or, where that is NULL, the *_all
+ * value of every row. */
+typedef struct kvm_sample_desc {
+  kvm_logits logits;
+  const float *uniforms;    /* [rows], in [0, 1) (values outside are clamped) */
+  const float *temperature; /* [rows] or NULL */
+  const int32_t *top_k;
+  const float *top_p;
+  const float *min_p;
+  double temperature_all;
+  int64_t top_k_all;
+  double top_p_all;
+  double min_p_all;
+  int64_t *tokens;          /* out [rows] */
+  float *logprobs;          /* out [rows] or NULL */
+} kvm_sample_desc;
+
+int kvm_sample(const kvm_sample_desc *d, void *stream);
+
+/* A loss on logits and its gradient, row by row:
+ *   loss = (1 - a) T^2 [sum_k p_k ln(p_k / q_k) + r ln(r / s)] + a [LSE(x) - x_label]
+ * p, r: the softmax over the teacher's k values / T and t_rest (r = 0 without
+ * t_rest); q_k, s: the student's probabilities at T of the same tokens and of
+ * all others together.  a = label_weight where there are labels, else 0;
+ * k = 0 (no teacher): the hard-label term alone, a = 1.
+ * Teacher entries whose index is outside [0, vocab) are padding; entries of
+ * the same token add up; a row of padding without t_rest has no soft term.
+ * Rows whose label is ignore_index have loss 0 and gradient 0; any other label
+ * outside [0, vocab) makes its row's loss and gradient NaN.
+ * grad (optional, the logits' type, strides g_outer / g_inner, starting at the
+ * same byte offset modulo 16 as the logits' row, for every row) receives
+ * d loss / d x, times *inv_count where inv_count is given.  inv_count
+ * (optional, written first): 1 / max(1, rows that count).  loss (optional):
+ * the sum of row_loss, times *inv_count where that is given. */
+typedef struct kvm_head_loss_desc {
+  kvm_logits logits;
+  const int64_t *labels;    /* [rows] or NULL (needs a teacher) */
+  int64_t ignore_index;
+  double label_weight;
+  int64_t k;                /* teacher entries per row, 0..1024 */
+  const void *t_values;     /* [rows, k] of t_dtype */
+  int64_t t_dtype;
+  const int64_t *t_indices; /* [rows, k] */
+  const float *t_rest;      /* [rows] or NULL */
+  double temperature;
+  float *row_loss;          /* out [rows] */
+  float *inv_count;         /* out [1] or NULL */
+  float *loss;              /* out [1] or NULL */
+  void *grad;               /* out or NULL */
+  int64_t g_outer, g_inner;
+} kvm_head_loss_desc;
+
+int kvm_head_loss(const kvm_head_loss_desc *d, void *stream);
+
+/* rows->data (written in place) times factor[r * factor_stride] of its row r
+ * (stride 0: one factor for all), products in fp32, rounded once; rows whose
+ * factor is 1 are not touched.  The backward of kvm_head_loss for an upstream
+ * gradient other than one. */
+int kvm_scale_rows(const kvm_logits *rows, const float *factor, int64_t factor_stride, void *stream);
+
 /* ABI self-description, checked by the host binding at load time. */
 int kvm_abi_version(void);
 int64_t kvm_struct_size(int which); /* 0 layer, 1 seq, 2 state, 3 prefill_desc, 4 prefix_desc,
-                                        5 prefill_bwd_desc, 6 state_bwd_desc, 7 add_norm_desc */
+                                        5 prefill_bwd_desc, 6 state_bwd_desc, 7 add_norm_desc, 8 logits,
+                                        10 sample_desc, 11 head_loss_desc */
 const char *kvm_last_error(void);
 
 /* Workspace of kvm_prefill for the given descriptor (snapshot_ring and

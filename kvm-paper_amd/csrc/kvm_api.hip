@@ -6,6 +6,7 @@
 #include <stdlib.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "kvm_internal.hpp"
@@ -60,6 +61,19 @@ int check_layer(const kvm_layer *L) {
   if (!L->ln_weight || !L->ln_bias || !L->state_temp || !L->front_temp)
     return fail(KVM_EINVAL, "layer parameter pointers must be set");
   if (!(L->ln_eps > 0.0)) return fail(KVM_EINVAL, "ln_eps must be positive");
+  return KVM_OK;
+}
+
+int check_logits(const kvm_logits *L, const char *what) {
+  if (!L || !L->data) return fail(KVM_EINVAL, "%s: logits must be set", what);
+  if (L->dtype < KVM_BF16 || L->dtype > KVM_F32) return fail(KVM_EINVAL, "%s: unknown logits type", what);
+  if (L->vocab < 1 || L->vocab > kvm::kMaxVocab)
+    return fail(KVM_EINVAL, "%s: vocab must be in [1, %lld], got %lld", what, (long long)kvm::kMaxVocab,
+                (long long)L->vocab);
+  if (L->outer < 1 || L->inner < 1 || L->outer > INT32_MAX || L->inner > INT32_MAX || L->outer * L->inner > INT32_MAX)
+    return fail(KVM_EINVAL, "%s: rows must be in [1, 2^31)", what);
+  if (reinterpret_cast<uintptr_t>(L->data) % (L->dtype == KVM_F32 ? 4 : 2))
+    return fail(KVM_EINVAL, "%s: logits must be aligned to their type", what);
   return KVM_OK;
 }
 
@@ -192,6 +206,9 @@ int64_t kvm_struct_size(int which) {
     case 5: return sizeof(kvm_prefill_bwd_desc);
     case 6: return sizeof(kvm_state_bwd_desc);
     case 7: return sizeof(kvm_add_norm_desc);
+    case 8: return sizeof(kvm_logits);
+    case 10: return sizeof(kvm_sample_desc);
+    case 11: return sizeof(kvm_head_loss_desc);
     default: return -1;
   }
 }
@@ -232,6 +249,73 @@ int kvm_add_norm(const kvm_add_norm_desc *d, void *stream) {
     if (p && !aligned16(p)) return fail(KVM_EINVAL, "add_norm pointers must be 16-byte aligned");
   if (!(P.eps >= 0.0)) return fail(KVM_EINVAL, "add_norm: eps must be >= 0");
   KVM_HIP(kvm::launch_add_norm(P, as_stream(stream)), "add_norm");
+  return KVM_OK;
+}
+
+int kvm_top_logits(const kvm_logits *logits, int64_t k, double temperature, void *values, int64_t *indices,
+                   float *rest, void *stream) {
+  if (const int rc = check_logits(logits, "top_logits")) return rc;
+  if (k < 1 || k > logits->vocab || k > kvm::top_logits_max())
+    return fail(KVM_EINVAL, "top_logits: k must be in [1, min(vocab, %lld)], got %lld",
+                (long long)kvm::top_logits_max(), (long long)k);
+  if (!(temperature > 0.0) || !std::isfinite(temperature))
+    return fail(KVM_EINVAL, "top_logits: temperature must be positive and finite");
+  if (!values || !indices) return fail(KVM_EINVAL, "top_logits: values and indices must be set");
+  KVM_HIP(kvm::launch_top_logits(*logits, k, temperature, values, indices, rest, as_stream(stream)), "top_logits");
+  return KVM_OK;
+}
+
+int kvm_sample(const kvm_sample_desc *d, void *stream) {
+  if (!d) return fail(KVM_EINVAL, "sample: NULL descriptor");
+  if (const int rc = check_logits(&d->logits, "sample")) return rc;
+  if (!d->uniforms || !d->tokens) return fail(KVM_EINVAL, "sample: uniforms and tokens must be set");
+  if (!d->temperature && !(d->temperature_all >= 0.0 && std::isfinite(d->temperature_all)))
+    return fail(KVM_EINVAL, "sample: temperature must be >= 0 and finite");
+  if (!d->top_k && (d->top_k_all < 0 || d->top_k_all > INT32_MAX))
+    return fail(KVM_EINVAL, "sample: top_k must be >= 0 (0: off)");
+  if (!d->top_p && !(d->top_p_all > 0.0 && d->top_p_all <= 1.0))
+    return fail(KVM_EINVAL, "sample: top_p must be in (0, 1]");
+  if (!d->min_p && !(d->min_p_all >= 0.0 && d->min_p_all <= 1.0))
+    return fail(KVM_EINVAL, "sample: min_p must be in [0, 1]");
+  KVM_HIP(kvm::launch_sample(*d, as_stream(stream)), "sample");
+  return KVM_OK;
+}
+
+int kvm_head_loss(const kvm_head_loss_desc *d, void *stream) {
+  if (!d) return fail(KVM_EINVAL, "head_loss: NULL descriptor");
+  const kvm_head_loss_desc &P = *d;
+  if (const int rc = check_logits(&P.logits, "head_loss")) return rc;
+  if (P.k < 0 || P.k > kvm::head_loss_max_teacher())
+    return fail(KVM_EINVAL, "head_loss: teacher entries per row must be in [0, %lld], got %lld",
+                (long long)kvm::head_loss_max_teacher(), (long long)P.k);
+  if (!P.row_loss) return fail(KVM_EINVAL, "head_loss: row_loss must be set");
+  if (P.k == 0 && !P.labels) return fail(KVM_EINVAL, "head_loss needs labels, a teacher, or both");
+  if (P.k > 0) {
+    if (!P.t_values || !P.t_indices) return fail(KVM_EINVAL, "head_loss: teacher values and indices must be set");
+    if (P.t_dtype < KVM_BF16 || P.t_dtype > KVM_F32) return fail(KVM_EINVAL, "head_loss: unknown teacher type");
+    if (!(P.temperature > 0.0) || !std::isfinite(P.temperature))
+      return fail(KVM_EINVAL, "head_loss: temperature must be positive and finite");
+    if (!(P.label_weight >= 0.0 && P.label_weight <= 1.0))
+      return fail(KVM_EINVAL, "head_loss: label_weight must be in [0, 1]");
+    if (P.label_weight > 0.0 && !P.labels) return fail(KVM_EINVAL, "head_loss: label_weight needs labels");
+  }
+  if (P.grad) {
+    if (P.grad == P.logits.data) return fail(KVM_EINVAL, "head_loss: grad may not be the logits");
+    // Same offset modulo 16 bytes in every row: the gradient is stored in the chunks the logits are read in.
+    const int64_t size = P.logits.dtype == KVM_F32 ? 4 : 2;
+    const bool outer = P.logits.outer > 1, inner = P.logits.inner > 1;
+    if ((reinterpret_cast<uintptr_t>(P.grad) - reinterpret_cast<uintptr_t>(P.logits.data)) % 16 ||
+        (outer && (P.g_outer - P.logits.s_outer) * size % 16) || (inner && (P.g_inner - P.logits.s_inner) * size % 16))
+      return fail(KVM_EINVAL, "head_loss: rows of grad must start at the offset modulo 16 bytes of the logits' rows");
+  }
+  KVM_HIP(kvm::launch_head_loss(P, as_stream(stream)), "head_loss");
+  return KVM_OK;
+}
+
+int kvm_scale_rows(const kvm_logits *rows, const float *factor, int64_t factor_stride, void *stream) {
+  if (const int rc = check_logits(rows, "scale_rows")) return rc;
+  if (!factor || factor_stride < 0) return fail(KVM_EINVAL, "scale_rows: factor must be set, its stride >= 0");
+  KVM_HIP(kvm::launch_scale_rows(*rows, factor, factor_stride, as_stream(stream)), "scale_rows");
   return KVM_OK;
 }
 

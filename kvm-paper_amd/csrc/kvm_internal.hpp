@@ -247,6 +247,15 @@ int gemm_small_tile_rows(int64_t M, int64_t N);
 // Residual add + LayerNorm + token shift of the decoder block (kvm_block.hip).
 hipError_t launch_add_norm(const kvm_add_norm_desc &P, hipStream_t stream);
 hipError_t launch_prefix(const kvm_prefix_desc &P, hipStream_t stream);
+// Operators on logits (kvm_sample.hip, kvm_loss.hip).
+constexpr int64_t kMaxVocab = 1 << 20;
+int64_t top_logits_max();
+hipError_t launch_top_logits(const kvm_logits &L, int64_t k, double temperature, void *values, int64_t *indices,
+                             float *rest, hipStream_t stream);
+hipError_t launch_sample(const kvm_sample_desc &P, hipStream_t stream);
+int64_t head_loss_max_teacher();
+hipError_t launch_head_loss(const kvm_head_loss_desc &P, hipStream_t stream);
+hipError_t launch_scale_rows(const kvm_logits &L, const float *up, int64_t up_st, hipStream_t stream);
 hipError_t launch_token_shift(const void *x, const void *prev, const void *mix, void *out, int64_t B,
                               int64_t T, int64_t width, int zero_fallback, hipStream_t stream);
 hipError_t launch_relu_square(const void *x, void *out, int64_t n, hipStream_t stream);

@@ -1,0 +1,218 @@
+// Rows of logits held by one workgroup (gfx950, wave64): loading, passes over
+// the values, and workgroup reductions.  Shared by the kernels that work on
+// whole rows [vocab] of a decoder's logits (kvm_sample.hip, kvm_loss.hip).
+//
+// A row is cut into 16-byte chunks that are aligned in memory; chunk c belongs
+// to thread c % T.  The up to N - 1 values before the first chunk and after the
+// last one (odd vocabularies and views that start anywhere) are held one per
+// lane of the first wave, so that no load touches memory outside the row.
+#pragma once
+
+#include "kvm_device.hpp"
+#include "kvm_internal.hpp"
+
+namespace kvm {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -__builtin_inff();
+
+// 16-byte chunks of the three value types <-> floats.
+template <int DT>
+struct Elem;
+template <>
+struct Elem<KVM_BF16> {
+  using raw = uint16_t;
+  static constexpr int N = 8;
+  static __device__ __forceinline__ float get(raw b) { return bf2f(b); }
+  static __device__ __forceinline__ raw put(float f) { return raw(f2bf(f)); }
+  static __device__ __forceinline__ void unpack(const uint4 u, float (&x)[N]) { unpack8(u, x); }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[N]) { return pack8(x); }
+};
+template <>
+struct Elem<KVM_F16> {
+  using raw = uint16_t;
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  static constexpr int N = 8;
+  static __device__ __forceinline__ float get(raw b) { return float(__builtin_bit_cast(_Float16, b)); }
+  static __device__ __forceinline__ raw put(float f) { return __builtin_bit_cast(raw, _Float16(f)); }
+  static __device__ __forceinline__ void unpack(const uint4 u, float (&x)[N]) {
+    const h8 h = __builtin_bit_cast(h8, u);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = float(h[i]);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[N]) {
+    h8 h;
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = _Float16(x[i]);
+    return __builtin_bit_cast(uint4, h);
+  }
+};
+template <>
+struct Elem<KVM_F32> {
+  using raw = float;
+  static constexpr int N = 4;
+  static __device__ __forceinline__ float get(raw b) { return b; }
+  static __device__ __forceinline__ raw put(float f) { return f; }
+  static __device__ __forceinline__ void unpack(const uint4 u, float (&x)[N]) {
+    x[0] = __uint_as_float(u.x);
+    x[1] = __uint_as_float(u.y);
+    x[2] = __uint_as_float(u.z);
+    x[3] = __uint_as_float(u.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&x)[N]) {
+    return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+  }
+};
+
+// First value of row r of a logits descriptor.
+template <int DT>
+__device__ __forceinline__ const typename Elem<DT>::raw *logits_row(const kvm_logits &L, int r) {
+  const int o = r / int(L.inner), i = r - o * int(L.inner);
+  return static_cast<const typename Elem<DT>::raw *>(L.data) + o * L.s_outer + i * L.s_inner;
+}
+
+// Sum / maximum over a wave, the same value in every lane (fixed order).
+__device__ __forceinline__ float lane_of(float v, int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+__device__ __forceinline__ float wave_add(float v) {
+  v = group_sum<16>(v);
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp<kDppRowRor8>(v));
+  v = fmaxf(v, dpp<kDppRowRor4>(v));
+  v = fmaxf(v, dpp<kDppQuadXor2>(v));
+  v = fmaxf(v, dpp<kDppQuadXor1>(v));
+  return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
+}
+
+// A row of V values in the registers of a workgroup of T threads, NV chunks
+// per thread (NV = 0: read again on every pass; for rows that do not fit).
+template <int DT, int T, int NV>
+struct Row {
+  using E = Elem<DT>;
+  using raw = typename E::raw;
+  static constexpr int N = E::N;
+  static constexpr int kBatch = 4;  // chunks of a thread in flight together when the row is read again
+
+  uint4 v[NV > 0 ? NV : 1];
+  const uint4 *chunks;
+  int head, nfull, edges;  // values before the first chunk, whole chunks, values outside them
+  int edge_idx;            // this lane's value outside the chunks (-1: none)
+  float edge;
+
+  __device__ __forceinline__ uint4 fetch(int c) const {
+    const uint4 u = chunks[min(c, nfull - 1)];
+    return u;
+  }
+  static __device__ __forceinline__ uint4 empty() {
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = kNegInf;
+    return E::pack(x);
+  }
+
+  __device__ __forceinline__ void open(const raw *row, int V) {
+    const int t = threadIdx.x;
+    const int mis = int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(raw));
+    head = mis ? min(N - mis, V) : 0;
+    nfull = (V - head) / N;
+    edges = V - nfull * N;
+    chunks = reinterpret_cast<const uint4 *>(row + head);
+    if constexpr (NV > 0) {
+      if (nfull > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) v[j] = fetch(j * T + t);
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (j * T + t >= nfull) v[j] = empty();
+    }
+    edge_idx = t < head ? t : head + nfull * N + (t - head);
+    if (t >= edges) edge_idx = -1;
+    edge = edge_idx >= 0 ? E::get(row[edge_idx]) : kNegInf;
+  }
+
+  // Position of value idx in an array that is laid out as the chunks are:
+  // the first value of every chunk lies at a multiple of N.
+  __device__ __forceinline__ int shifted(int idx) const { return idx + (head ? N - head : 0); }
+
+  // f(x, first, n): n values x[0..n) with indices first, first + 1, ...  n is
+  // N, or 1 (a value outside the chunks), or 0 (none); the values past n are
+  // -infinity.  Chunks that no lane of the workgroup has are skipped.
+  template <class F>
+  __device__ __forceinline__ void each(F &&f) const {
+    const int t = threadIdx.x;
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (j * T < nfull) {
+          float x[N];
+          E::unpack(v[j], x);
+          const int c = j * T + t;
+          f(x, head + c * N, c < nfull ? N : 0);
+        }
+      }
+    } else {
+      for (int c0 = t; c0 - t < nfull; c0 += T * kBatch) {
+        uint4 u[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) u[i] = fetch(c0 + i * T);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int c = c0 + i * T;
+          if (c - t < nfull) {
+            float x[N];
+            E::unpack(c < nfull ? u[i] : empty(), x);
+            f(x, head + c * N, c < nfull ? N : 0);
+          }
+        }
+      }
+    }
+    if (edges && t < kWave) {
+      float x[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = kNegInf;
+      x[0] = edge;
+      f(x, edge_idx, edge_idx >= 0 ? 1 : 0);
+    }
+  }
+};
+
+// What a launch takes for rows of a type and length: threads per workgroup,
+// and whether the row stays in registers.  16 chunks per thread are 64
+// registers, which leaves two workgroups of 512 threads (or one of 1024) per
+// compute unit; longer rows are read again on every pass, from the caches.
+constexpr int kRowChunks = 16;
+inline int row_threads(int64_t vocab, int64_t dtype, int64_t at_least = 256) {
+  const int64_t n = dtype == KVM_F32 ? 4 : 8;
+  int64_t t = 256;
+  while (t < 1024 && (t < at_least || t * kRowChunks * n < vocab)) t *= 2;
+  return int(t);
+}
+inline bool row_resident(int64_t vocab, int64_t dtype) {
+  return vocab <= int64_t(1024) * kRowChunks * (dtype == KVM_F32 ? 4 : 8);
+}
+
+// Calls f.template operator()<DT, T, NV>() for the variant of a row.
+template <class F>
+void with_row(int64_t vocab, int64_t dtype, int64_t at_least, F &&f) {
+  const int t = row_threads(vocab, dtype, at_least);
+  const bool res = row_resident(vocab, dtype);
+#define KVM_ROW_DT(D)                                       \
+  if (!res) f.template run<D, 1024, 0>();                   \
+  else if (t == 256) f.template run<D, 256, kRowChunks>();  \
+  else if (t == 512) f.template run<D, 512, kRowChunks>();  \
+  else f.template run<D, 1024, kRowChunks>();
+  if (dtype == KVM_BF16) {
+    KVM_ROW_DT(KVM_BF16)
+  } else if (dtype == KVM_F16) {
+    KVM_ROW_DT(KVM_F16)
+  } else {
+    KVM_ROW_DT(KVM_F32)
+  }
+#undef KVM_ROW_DT
+}
+
+}  // namespace kvm

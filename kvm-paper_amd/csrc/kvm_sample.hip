@@ -1,0 +1,688 @@
+// The largest logits of a row, and sampling from a row of logits, on gfx950.
+//
+// Both rank a row's V logits x by (value falling, index rising); -0 equals +0
+// and a NaN counts as -infinity.
+//
+// Top logits: the K first of that order, and the log-sum-exp of x_i / T over
+// all others.
+//
+// Sampling at a temperature T: token j of the order has the whole-number weight
+//   w_j = floor(2^42 exp((x_j - x_0) / T) + 1/2),
+// so that every sum below is exact in 64 bits, whatever its order, and atomic
+// additions cannot change a result (V <= 2^20 keeps a sum below 2^62).  Top-k
+// keeps the first k tokens, top-p of these the shortest prefix with at least
+// p of their weight, min-p of these the tokens with w_j >= min_p 2^42.  Each
+// keeps a prefix of the order, so what is kept is told by its weight C alone,
+// and the token drawn with the uniform number u is the first whose running sum
+// passes floor(u C).  A row is never sorted: all that is needed is to find the
+// token at a given running sum (or rank), "locating" it.
+//
+// Locating, in general: a histogram of weights (or counts) over 2048 bins that
+// are linear in (x_0 - x) / T up to the 43 ln 2 past which weights are zero; a
+// prefix sum over it names the bin; the bin's tokens (about 50 for logits with
+// a spread of a few nats) are collected and ranked by counting, each against
+// each.  A bin with more than 1024 tokens is cut again by their bit patterns
+// until it has fewer, or holds one value only, whose tokens rank by index.
+//
+// Locating, for k up to half the workgroup: the k-th largest of the threads'
+// own maxima is a lower bound of the k-th largest logit that few other logits
+// pass (T ln(1 / (1 - k/T)) for T threads and logits in no particular order);
+// those that do are collected and ranked by counting.
+//
+// One workgroup per row.  The top logits hold the row in registers; sampling
+// reads it again on every pass, from the caches, in loops that are not unrolled
+// (with the fp64 exponentials in them they would not fit the instruction cache).
+
+#include "kvm_rows.hpp"
+
+namespace kvm {
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int kBins = 2048;
+constexpr int kCand = 1024;        // tokens that are ranked by counting
+constexpr int kSampleThreads = 1024;
+constexpr int kMaxTop = 512;       // K of the top logits
+constexpr double kUnit = 4398046511104.0;  // 2^42
+
+// Bit patterns in the order of the values: larger float, larger key.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  const uint32_t b = __float_as_uint(fmaxf(x, kNegInf) + 0.f);  // NaN -> -infinity, -0 -> +0
+  return (b >> 31) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
+}
+// The order of a row as one number: larger first.
+__device__ __forceinline__ u64 rank_of(uint32_t key, int idx) { return u64(key) << 32 | (0xffffffffu - uint32_t(idx)); }
+__device__ __forceinline__ int index_of(u64 rank) { return int(0xffffffffu - uint32_t(rank)); }
+__device__ __forceinline__ uint32_t key_part(u64 rank) { return uint32_t(rank >> 32); }
+
+// 2^y for y <= 0 in fp64, relative error below 2^-50: 2^n times the Taylor
+// series of 2^f = exp(f ln 2), |f| <= 1/2, to the twelfth power.
+// No contraction: a token's weight is the same wherever it is computed.
+__device__ __forceinline__ double exp2_wide(double y) {
+#pragma clang fp contract(off)
+  const double n = rint(y), f = (y - n) * 0.6931471805599453;
+  double p = 1.0 / 479001600.0;
+  p = __builtin_fma(p, f, 1.0 / 39916800.0);
+  p = __builtin_fma(p, f, 1.0 / 3628800.0);
+  p = __builtin_fma(p, f, 1.0 / 362880.0);
+  p = __builtin_fma(p, f, 1.0 / 40320.0);
+  p = __builtin_fma(p, f, 1.0 / 5040.0);
+  p = __builtin_fma(p, f, 1.0 / 720.0);
+  p = __builtin_fma(p, f, 1.0 / 120.0);
+  p = __builtin_fma(p, f, 1.0 / 24.0);
+  p = __builtin_fma(p, f, 1.0 / 6.0);
+  p = __builtin_fma(p, f, 0.5);
+  p = __builtin_fma(p, f, 1.0);
+  p = __builtin_fma(p, f, 1.0);
+  return ldexp(p, int(n));
+}
+
+// Weights and bins of a row at one temperature.
+struct Weights {
+  float best;      // x_0
+  double log2_per; // log2(e) / T
+  float bins_per;  // bins per unit of logit
+  __device__ __forceinline__ u64 operator()(float x) const {
+#pragma clang fp contract(off)
+    if (x == best) return u64(kUnit);
+    const double y = (double(x) - double(best)) * log2_per;
+    if (!(y >= -43.0)) return 0;
+    // 2^42 e + 1/2 is below 2^43: adding 2^52 to the product rounds it to a
+    // whole number in the low bits.
+    return __builtin_bit_cast(u64, __builtin_fma(exp2_wide(y), kUnit, 4503599627370496.0)) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ int bin(float x) const {
+    const float d = x == best ? 0.f : best - x;
+    return int(fminf(fmaxf(d * bins_per, 0.f), float(kBins - 1)));  // NaN (0 times infinity): 0
+  }
+};
+
+struct Shared {
+  u64 hist[kBins];
+  u64 fine[kBins];
+  u64 cand[kCand];
+  u64 cw[kCand];
+  u64 scan[17];
+  float red[16];
+  int ired[16];
+  uint32_t kmin, kmax;
+  int count, bin;
+  u64 base;        // weight (or count) before the located bin
+  u64 found;       // the located token (its rank_of)
+  u64 found_end;   // running sum including it
+  uint32_t bound;
+};
+
+template <int T>
+__device__ __forceinline__ float block_max(float v, float *red) {
+  v = wave_max(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < T / kWave; ++w) v = fmaxf(v, red[w]);
+  return v;
+}
+template <int T>
+__device__ __forceinline__ int block_min(int v, int *red) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = min(v, __shfl_xor(v, o));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < T / kWave; ++w) v = min(v, red[w]);
+  return v;
+}
+template <int T>
+__device__ __forceinline__ u64 block_add(u64 v, u64 *red) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < T / kWave; ++w) v += red[w];
+  return v;
+}
+// Exclusive prefix sum over the workgroup's threads; *total its end.
+template <int T>
+__device__ __forceinline__ u64 block_scan(u64 v, u64 *red, u64 *total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  u64 s = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const u64 up = __shfl_up(s, o);
+    if (lane >= o) s += up;
+  }
+  __syncthreads();
+  if (lane == 63) red[wave] = s;
+  __syncthreads();
+  u64 before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < T / kWave; ++w) {
+    if (w < wave) before += red[w];
+    all += red[w];
+  }
+  *total = all;
+  return before + s - v;
+}
+
+// Collects the values of a row with keys >= bound (in no particular order)
+// and returns how many there are; the list holds the first kCand of them.
+template <int T, class R>
+__device__ __forceinline__ int collect_above(const R &x, uint32_t bound, Shared &sh) {
+  constexpr int N = R::N;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  const float least = value_of(bound);
+  x.each([&](const float (&v)[N], int i0, int n) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
+    if (!(m < least)) {  // a NaN row part comes here too and is compared by key
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t k = key_of(v[i]);
+        if (i < n && k >= bound) {
+          const int at = atomicAdd(&sh.count, 1);
+          if (at < kCand) sh.cand[at] = rank_of(k, i0 + i);
+        }
+      }
+    }
+  });
+  __syncthreads();
+  return sh.count;
+}
+
+// A lower bound of the k-th largest key of the row: (about) the k-th largest
+// of the threads' maxima, found by bisection in the first wave.  T >= k.
+template <int T, class R>
+__device__ __forceinline__ uint32_t bound_of(float thread_max, int k, Shared &sh) {
+  uint32_t *keys = reinterpret_cast<uint32_t *>(sh.fine);
+  const int t = threadIdx.x;
+  keys[t] = key_of(thread_max);
+  __syncthreads();
+  if (t < kWave) {
+    constexpr int M = T / kWave;
+    uint32_t mine[M], lo = 0xffffffffu, hi = 0;
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      mine[i] = keys[i * kWave + t];
+      lo = min(lo, mine[i]);
+      hi = max(hi, mine[i]);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      lo = min(lo, uint32_t(__shfl_xor(int(lo), o)));
+      hi = max(hi, uint32_t(__shfl_xor(int(hi), o)));
+    }
+    // Invariant: at least k keys are >= lo.  An interval that passes a few
+    // more than k keys is good enough.
+    const int enough = k + k / 8;
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < M; ++i) c += __popcll(__ballot(mine[i] >= mid));
+      if (c >= k) {
+        lo = mid;
+        if (c <= enough) break;
+      } else {
+        hi = mid;
+      }
+    }
+    if (t == 0) sh.bound = lo;
+  }
+  __syncthreads();
+  return sh.bound;
+}
+
+// The token at running sum `target` (before <= target < before + its own) in
+// the order of the row, of weights (COUNT: of ones).  hist: the quantity per
+// bin of the row, which has been built; mine: this thread's exclusive prefix of
+// it.  Writes sh.found and sh.found_end.  in(x) selects values with a positive
+// quantity; every thread gets here.
+template <int T, bool COUNT, class R, class In>
+__device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target, u64 mine, Shared &sh, In &&in) {
+  constexpr int N = R::N, PER = kBins / T;
+  const int t = threadIdx.x;
+  // the bin
+  __syncthreads();
+  {
+    u64 s = mine;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const u64 q = sh.hist[t * PER + i];
+      if (target >= s && target < s + q) {
+        sh.bin = t * PER + i;
+        sh.base = s;
+      }
+      s += q;
+    }
+  }
+  if (t == 0) {
+    sh.count = 0;
+    sh.kmin = 0xffffffffu;
+    sh.kmax = 0;
+  }
+  __syncthreads();
+  const int bin = sh.bin;
+  u64 base = sh.base;
+  uint32_t lo = 0, hi = 0xffffffffu;  // keys of the tokens in question
+  bool first = true;
+  uint32_t f_hi = 0, f_span = 0;
+  int f_bin = 0;
+  while (true) {
+    // collect the tokens of the (sub-)bin, with their smallest and largest key
+    uint32_t a = 0xffffffffu, b = 0;
+    x.each([&](const float (&v)[N], int i0, int n) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i < n) {
+          const uint32_t k = key_of(v[i]);
+          const float xv = value_of(k);
+          bool hit = k >= lo && k <= hi && wt.bin(xv) == bin;
+          if (hit && !first) hit = int(u64(f_hi - k) * kBins / (u64(f_span) + 1)) == f_bin;
+          if (hit && in(xv, i0 + i)) {
+            a = min(a, k);
+            b = max(b, k);
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kCand) sh.cand[at] = rank_of(k, i0 + i);
+          }
+        }
+      }
+    });
+    if (a <= b) {
+      atomicMin(&sh.kmin, a);
+      atomicMax(&sh.kmax, b);
+    }
+    __syncthreads();
+    const int cnt = sh.count;
+    lo = sh.kmin;
+    hi = sh.kmax;
+    if (cnt <= kCand) {
+      for (int i = t; i < cnt; i += T) sh.cw[i] = COUNT ? 1 : wt(value_of(key_part(sh.cand[i])));
+      __syncthreads();
+      for (int i = t; i < cnt; i += T) {
+        const u64 me = sh.cand[i];
+        u64 before = base;
+        for (int j = 0; j < cnt; ++j)
+          if (sh.cand[j] > me) before += sh.cw[j];
+        if (target >= before && target < before + sh.cw[i]) {
+          sh.found = me;
+          sh.found_end = before + sh.cw[i];
+        }
+      }
+      __syncthreads();
+      return;
+    }
+    if (lo == hi) {
+      // One value: the n-th of its tokens by index, found by bisection over the index.
+      const u64 w = COUNT ? 1 : wt(value_of(lo));
+      const u64 nth = (target - base) / w;
+      int below = -1, upto = (1 << 20) - 1;  // at most nth tokens are <= below, more than nth are <= upto
+      while (upto - below > 1) {
+        const int mid = below + (upto - below) / 2;
+        u64 c = 0;
+        x.each([&](const float (&v)[N], int i0, int n) {
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (i < n && i0 + i <= mid && key_of(v[i]) == lo && in(v[i], i0 + i)) ++c;
+        });
+        c = block_add<T>(c, sh.scan);
+        if (c > nth)
+          upto = mid;
+        else
+          below = mid;
+      }
+      if (t == 0) {
+        sh.found = rank_of(lo, upto);
+        sh.found_end = base + (nth + 1) * w;
+      }
+      __syncthreads();
+      return;
+    }
+    // cut [lo, hi] into kBins by key, the largest keys first
+    __syncthreads();
+    for (int i = t; i < kBins; i += T) sh.fine[i] = 0;
+    f_hi = hi;
+    f_span = hi - lo;
+    __syncthreads();
+    x.each([&](const float (&v)[N], int i0, int n) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t k = key_of(v[i]);
+        const float xv = value_of(k);
+        if (i < n && k >= lo && k <= hi && wt.bin(xv) == bin && in(xv, i0 + i))
+          atomicAdd(&sh.fine[int(u64(f_hi - k) * kBins / (u64(f_span) + 1))], COUNT ? 1 : wt(xv));
+      }
+    });
+    __syncthreads();
+    u64 own = 0, all;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) own += sh.fine[t * PER + i];
+    u64 s = base + block_scan<T>(own, sh.scan, &all);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const u64 q = sh.fine[t * PER + i];
+      if (target >= s && target < s + q) {
+        sh.bin = t * PER + i;
+        sh.base = s;
+      }
+      s += q;
+    }
+    if (t == 0) {
+      sh.count = 0;
+      sh.kmin = 0xffffffffu;
+      sh.kmax = 0;
+    }
+    __syncthreads();
+    f_bin = sh.bin;
+    base = sh.base;
+    first = false;
+  }
+}
+
+// Histogram of a row's weights (COUNT: of ones) over the values that in()
+// selects; returns this thread's exclusive prefix, *total the sum.  strong
+// (optional): the sum of the weights >= least.
+template <int T, bool COUNT, class R, class In>
+__device__ __forceinline__ u64 build(const R &x, const Weights &wt, Shared &sh, u64 *total, double least, u64 *strong,
+                                     In &&in) {
+  constexpr int N = R::N, PER = kBins / T;
+  const int t = threadIdx.x;
+  __syncthreads();
+  for (int i = t; i < kBins; i += T) sh.hist[i] = 0;
+  __syncthreads();
+  u64 big = 0;
+  x.each([&](const float (&v)[N], int i0, int n) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i < n && in(v[i], i0 + i)) {
+        const u64 w = wt(v[i]);
+        if (w) {
+          atomicAdd(&sh.hist[wt.bin(v[i])], COUNT ? 1 : w);
+          if (strong && double(w) >= least) big += w;
+        }
+      }
+    }
+  });
+  __syncthreads();
+  if (strong) *strong = block_add<T>(big, sh.scan);
+  u64 own = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) own += sh.hist[t * PER + i];
+  return block_scan<T>(own, sh.scan, total);
+}
+
+// floor(u * c) for a uniform number, inside [0, c - 1] whatever u is.
+__device__ __forceinline__ u64 target_of(float u, u64 c) {
+  const double at = floor(double(u) * double(c));
+  const u64 last = c - 1;
+  if (!(at > 0.0)) return 0;
+  return at >= double(last) ? last : u64(at);
+}
+
+template <int DT>
+__global__ __launch_bounds__(kSampleThreads) void k_sample(kvm_sample_desc P) {
+  constexpr int T = kSampleThreads;
+  using R = Row<DT, T, 0>;
+  constexpr int N = R::N;
+  __shared__ Shared sh;
+  const int t = threadIdx.x, row = blockIdx.x;
+  const int V = int(P.logits.vocab);
+  R x;
+  x.open(logits_row<DT>(P.logits, row), V);
+  const float temp = P.temperature ? P.temperature[row] : float(P.temperature_all);
+  float top_p = P.top_p ? P.top_p[row] : float(P.top_p_all);
+  float min_p = P.min_p ? P.min_p[row] : float(P.min_p_all);
+  top_p = top_p < 1.f ? top_p : 1.f;  // a NaN keeps everything
+  min_p = min_p > 0.f ? min_p : 0.f;
+  const int top_k = P.top_k ? P.top_k[row] : int(P.top_k_all);
+  const float u = P.uniforms[row];
+
+  float mine = kNegInf;
+  x.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine = fmaxf(mine, v[i]);
+  });
+  const float best = block_max<T>(mine, sh.red);
+  auto answer = [&](int token, float logprob) {  // one thread
+    P.tokens[row] = token;
+    if (P.logprobs) P.logprobs[row] = logprob;
+  };
+  if (best == kNegInf) {  // nothing to draw from
+    if (t == 0) answer(0, __builtin_nanf(""));
+    return;
+  }
+  if (!(temp > 0.f) || top_k == 1) {  // the first token of the order
+    int at = 0x7fffffff;
+    x.each([&](const float (&v)[N], int i0, int n) {
+#pragma unroll
+      for (int i = N - 1; i >= 0; --i)
+        if (i < n && v[i] == best) at = min(at, i0 + i);
+    });
+    at = block_min<T>(at, sh.ired);
+    if (t == 0) answer(at, 0.f);
+    return;
+  }
+  Weights wt;
+  wt.best = best;
+  wt.log2_per = 1.4426950408889634 / double(temp);
+  // 43 octaves of weight fill the bins
+  wt.bins_per = float(double(kBins) / (43.0 * 0.6931471805599453 * double(temp)));
+  const double least = double(min_p) * kUnit;
+  auto write = [&](u64 rank, u64 c) {  // one thread: the token and ln(w / C)
+    const float xv = value_of(key_part(rank));
+    const double d = xv == best ? 0.0 : (double(xv) - double(best)) / double(temp);
+    answer(index_of(rank), float(d - log(double(c) / kUnit)));
+  };
+
+  if (top_k > 0 && top_k <= T / 2 && top_k < V) {
+    const uint32_t bound = bound_of<T, R>(mine, top_k, sh);
+    const int cnt = collect_above<T>(x, bound, sh);
+    if (cnt <= kCand) {
+      const int k = min(top_k, cnt);
+      u64 *sorted = sh.hist;
+      for (int i = t; i < cnt; i += T) {
+        const u64 me = sh.cand[i];
+        int r = 0;
+        for (int j = 0; j < cnt; ++j) r += sh.cand[j] > me;
+        if (r < k) sorted[r] = me;
+      }
+      __syncthreads();
+      const u64 me = t < k ? sorted[t] : 0;  // k <= T / 2: one token per thread
+      const u64 w = t < k ? wt(value_of(key_part(me))) : 0;
+      u64 z;
+      const u64 before = block_scan<T>(w, sh.scan, &z);
+      const bool keep = t == 0 || (double(before) < double(top_p) * double(z) && double(w) >= least);
+      const u64 c = block_add<T>(keep ? w : 0, sh.scan);
+      const u64 at = target_of(u, c);
+      if (at >= before && at < before + w) write(me, c);
+      return;
+    }
+    __syncthreads();
+  }
+  auto all = [](float, int) { return true; };
+  u64 limit = 0;  // the last token that top-k keeps (0: it keeps all)
+  u64 z;
+  if (top_k > 0 && top_k < V) {
+    const u64 pre = build<T, true>(x, wt, sh, &z, 0.0, nullptr, all);
+    if (u64(top_k) < z) {
+      auto positive = [&](float v, int) { return wt(v) != 0; };
+      locate<T, true>(x, wt, u64(top_k) - 1, pre, sh, positive);
+      limit = sh.found;
+    }
+  }
+  auto kept = [&](float v, int i) { return limit == 0 || rank_of(key_of(v), i) >= limit; };
+  u64 strong = 0;
+  const u64 pre = build<T, false>(x, wt, sh, &z, least, min_p > 0.f ? &strong : nullptr, kept);
+  auto weighted = [&](float v, int i) { return kept(v, i) && wt(v) != 0; };
+  u64 c = z;
+  if (top_p < 1.f) {
+    const double end = ceil(double(top_p) * double(z));
+    if (end >= 1.0) {
+      locate<T, false>(x, wt, u64(end) - 1, pre, sh, weighted);
+      c = sh.found_end;
+    } else {
+      c = 0;
+    }
+  }
+  if (min_p > 0.f && strong < c) c = strong;
+  if (c < u64(kUnit)) c = u64(kUnit);  // the first token is always kept
+  locate<T, false>(x, wt, target_of(u, c), pre, sh, weighted);
+  if (t == 0) write(sh.found, c);
+}
+
+template <int DT, int T, int NV>
+__global__ __launch_bounds__(T) void k_top_logits(kvm_logits L, int K, float scale, void *values, int64_t *indices,
+                                                  float *rest) {
+  using R = Row<DT, T, NV>;
+  using E = Elem<DT>;
+  constexpr int N = R::N;
+  __shared__ Shared sh;
+  __shared__ u64 s_last, s_next;
+  const int t = threadIdx.x, row = blockIdx.x;
+  const int V = int(L.vocab);
+  R x;
+  x.open(logits_row<DT>(L, row), V);
+  float mine = kNegInf;
+  x.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine = fmaxf(mine, v[i]);
+  });
+  if (t == 0) s_next = 0;
+  const uint32_t bound = bound_of<T, R>(mine, K, sh);
+  int cnt = collect_above<T>(x, bound, sh);
+  u64 more_ties = 0;  // tokens of the K-th value behind it that are not in the list
+  if (cnt > kCand) {
+    // Many equal or clustered logits: the K-th token by rank, then exactly K are collected.
+    Weights wt;  // one bin: the tokens are cut by their keys from the start
+    wt.best = 0.f;
+    wt.log2_per = 0.0;
+    wt.bins_per = 0.f;
+    __syncthreads();
+    for (int i = t; i < kBins; i += T) sh.hist[i] = i ? 0 : u64(V);
+    auto all = [](float, int) { return true; };
+    Row<DT, T, 0> again;
+    again.open(logits_row<DT>(L, row), V);
+    locate<T, true>(again, wt, u64(K) - 1, t ? u64(V) : 0, sh, all);
+    const u64 last = sh.found;
+    __syncthreads();
+    if (t == 0) sh.count = 0;
+    __syncthreads();
+    u64 ties = 0;
+    again.each([&](const float (&v)[N], int i0, int n) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i < n) {
+          const uint32_t k = key_of(v[i]);
+          const u64 me = rank_of(k, i0 + i);
+          if (me >= last) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kCand) sh.cand[at] = me;
+          } else if (k == key_part(last)) {
+            ++ties;
+          }
+        }
+      }
+    });
+    __syncthreads();
+    more_ties = block_add<T>(ties, sh.scan);
+    cnt = K;
+  }
+  u64 in_list = 0;
+  for (int i = t; i < cnt; i += T) {
+    const u64 me = sh.cand[i];
+    int r = 0;
+    for (int j = 0; j < cnt; ++j) r += sh.cand[j] > me;
+    if (r < K) {
+      static_cast<typename E::raw *>(values)[int64_t(row) * K + r] = E::put(value_of(key_part(me)));
+      indices[int64_t(row) * K + r] = index_of(me);
+    }
+    if (r == K - 1) s_last = me;
+    if (r == K) s_next = me;
+  }
+  if (!rest) return;
+  __syncthreads();
+  const u64 last = s_last, next = s_next;
+  const uint32_t kth = key_part(last);
+  for (int i = t; i < cnt; i += T) in_list += sh.cand[i] < last && key_part(sh.cand[i]) == kth;
+  const float ties = float(block_add<T>(in_list, sh.scan) + more_ties);
+  const float vk = value_of(kth);
+  // The largest of the others: behind the K-th in the list, or below the list's bound.
+  float m = kNegInf;
+  if (next) {
+    m = value_of(key_part(next));
+  } else if (K < V) {
+    x.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) m = fmaxf(m, v[i] < vk ? v[i] : kNegInf);
+    });
+    m = block_max<T>(m, sh.red);
+    if (ties > 0.f) m = vk;
+  }
+  const float ref = m == kNegInf ? 0.f : m;
+  float z = 0.f;
+  x.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      z += __builtin_amdgcn_exp2f(v[i] < vk ? (v[i] - ref) * scale : kNegInf);
+  });
+  z = wave_add(z);
+  __syncthreads();
+  if ((t & 63) == 0) sh.red[t >> 6] = z;
+  __syncthreads();
+  if (t == 0) {
+    z = ties;  // each of them is the reference itself: m = vk, exp = 1
+    for (int w = 0; w < T / kWave; ++w) z += sh.red[w];
+    const double lse = m == kNegInf ? -__builtin_inf() : (double(ref) * scale + log2(double(z))) * 0.6931471805599453;
+    rest[row] = float(lse);
+  }
+}
+
+struct TopLaunch {
+  const kvm_logits &L;
+  int K;
+  float scale;
+  void *values;
+  int64_t *indices;
+  float *rest;
+  hipStream_t stream;
+  template <int DT, int T, int NV>
+  void run() {
+    hipLaunchKernelGGL((k_top_logits<DT, T, NV>), dim3(unsigned(L.outer * L.inner)), dim3(T), 0, stream, L, K, scale,
+                       values, indices, rest);
+  }
+};
+
+}  // namespace
+
+int64_t top_logits_max() { return kMaxTop; }
+
+hipError_t launch_sample(const kvm_sample_desc &P, hipStream_t stream) {
+  const dim3 grid(unsigned(P.logits.outer * P.logits.inner)), block(kSampleThreads);
+  if (P.logits.dtype == KVM_BF16)
+    hipLaunchKernelGGL(k_sample<KVM_BF16>, grid, block, 0, stream, P);
+  else if (P.logits.dtype == KVM_F16)
+    hipLaunchKernelGGL(k_sample<KVM_F16>, grid, block, 0, stream, P);
+  else
+    hipLaunchKernelGGL(k_sample<KVM_F32>, grid, block, 0, stream, P);
+  return hipGetLastError();
+}
+
+hipError_t launch_top_logits(const kvm_logits &L, int64_t k, double temperature, void *values, int64_t *indices,
+                             float *rest, hipStream_t stream) {
+  TopLaunch l{L, int(k), float(1.4426950408889634 / temperature), values, indices, rest, stream};
+  // At least twice as many threads as values: the bound from the threads' maxima then passes 1.4 K logits or fewer.
+  with_row(L.vocab, L.dtype, 2 * k, l);
+  return hipGetLastError();
+}
+
+}  // namespace kvm

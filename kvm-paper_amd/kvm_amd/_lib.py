@@ -16,7 +16,7 @@ import torch
 
 LIB_NAME = "libkvm_amd.so"
 LIB_PATH = Path(__file__).resolve().parent / LIB_NAME
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 KVM_OK = 0
 KVM_EINVAL = -1
@@ -25,6 +25,7 @@ KVM_ESPACE = -3
 KVM_EABORT = -4
 KVM_STATUS_CHAIN_TIMEOUT = 1
 KVM_PREFILL_NO_CHAIN = 1
+KVM_BF16, KVM_F16, KVM_F32 = 0, 1, 2
 
 _i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
@@ -151,6 +152,33 @@ class KvmAddNormDesc(ctypes.Structure):
     ]
 
 
+class KvmLogits(ctypes.Structure):
+    _fields_ = [
+        ("data", _vp), ("dtype", _i64), ("vocab", _i64), ("outer", _i64), ("inner", _i64),
+        ("s_outer", _i64), ("s_inner", _i64),
+    ]
+
+
+class KvmSampleDesc(ctypes.Structure):
+    _fields_ = [
+        ("logits", KvmLogits), ("uniforms", _vp),
+        ("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp),
+        ("temperature_all", ctypes.c_double), ("top_k_all", _i64), ("top_p_all", ctypes.c_double),
+        ("min_p_all", ctypes.c_double),
+        ("tokens", _vp), ("logprobs", _vp),
+    ]
+
+
+class KvmHeadLossDesc(ctypes.Structure):
+    _fields_ = [
+        ("logits", KvmLogits), ("labels", _vp), ("ignore_index", _i64), ("label_weight", ctypes.c_double),
+        ("k", _i64), ("t_values", _vp), ("t_dtype", _i64), ("t_indices", _vp), ("t_rest", _vp),
+        ("temperature", ctypes.c_double),
+        ("row_loss", _vp), ("inv_count", _vp), ("loss", _vp),
+        ("grad", _vp), ("g_outer", _i64), ("g_inner", _i64),
+    ]
+
+
 # Exported symbols and their signatures (include/kvm_amd.h).
 _P = ctypes.POINTER
 SIGNATURES = {
@@ -177,6 +205,10 @@ SIGNATURES = {
     "kvm_gemm_small_tile_rows": (ctypes.c_int, [_i64, _i64]),
     "kvm_gemm_small_packed": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, ctypes.c_int,
                                              ctypes.c_int, _vp]),
+    "kvm_top_logits": (ctypes.c_int, [_P(KvmLogits), _i64, ctypes.c_double, _vp, _vp, _vp, _vp]),
+    "kvm_sample": (ctypes.c_int, [_P(KvmSampleDesc), _vp]),
+    "kvm_head_loss": (ctypes.c_int, [_P(KvmHeadLossDesc), _vp]),
+    "kvm_scale_rows": (ctypes.c_int, [_P(KvmLogits), _vp, _i64, _vp]),
     "kvm_state_append_direct": (ctypes.c_int, [_P(KvmLayer), _P(KvmSeq), _i64, _i64, _P(KvmState), _i64, _vp]),
     "kvm_state_refresh": (ctypes.c_int, [_P(KvmLayer), _P(KvmState), _i64, _i64, _vp]),
     "kvm_update_workspace_bytes": (_i64, [_P(KvmLayer), _i64]),
@@ -219,8 +251,10 @@ def load(path: str | os.PathLike | None = None):
         fn.argtypes = args
     if lib.kvm_abi_version() != ABI_VERSION:
         raise KvmLibraryError(f"{p}: ABI version {lib.kvm_abi_version()} != {ABI_VERSION}")
-    for i, st in enumerate((KvmLayer, KvmSeq, KvmState, KvmPrefillDesc, KvmPrefixDesc, KvmPrefillBwdDesc,
-                              KvmStateBwdDesc, KvmAddNormDesc)):
+    structs = dict(enumerate((KvmLayer, KvmSeq, KvmState, KvmPrefillDesc, KvmPrefixDesc, KvmPrefillBwdDesc,
+                              KvmStateBwdDesc, KvmAddNormDesc, KvmLogits)))
+    structs |= {10: KvmSampleDesc, 11: KvmHeadLossDesc}
+    for i, st in structs.items():
         if lib.kvm_struct_size(i) != ctypes.sizeof(st):
             raise KvmLibraryError(f"{p}: struct {st.__name__} size mismatch")
     if path is None:

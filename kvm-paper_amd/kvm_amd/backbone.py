@@ -42,6 +42,8 @@ from torch import nn
 
 from . import _lib
 from .linear import linear, module_linear
+from .logits import TopLogits, sample_tokens, top_logits
+from .losses import cross_entropy, distillation_loss
 from .mixer import SequenceMixer, set_label
 from .states_cache import StatesDictCache
 
@@ -561,16 +563,55 @@ class RWKV7BackboneForCausalLM(nn.Module):
                 inputs_embeds=None, labels=None, use_cache=None, logits_to_keep: int | torch.Tensor = 0,
                 **kwargs) -> CausalLMOutput:
         if labels is not None:
-            raise ValueError("this build runs the inference forward path only (no loss)")
+            raise ValueError("forward() is the inference path and computes no loss; call loss(input_ids, labels)")
         base = self.transformer(input_ids=input_ids, attention_mask=attention_mask, position_ids=position_ids,
                                 past_key_values=past_key_values, inputs_embeds=inputs_embeds, use_cache=use_cache,
                                 **kwargs)
         hidden, cache = base.last_hidden_state, base.past_key_values
         keep = slice(-logits_to_keep, None) if isinstance(logits_to_keep, int) else logits_to_keep
-        logits = module_linear(self.lm_head, hidden[:, keep, :])
+        return CausalLMOutput(logits=self._head(hidden[:, keep, :]).float(), past_key_values=cache)
+
+    def _head(self, hidden: torch.Tensor) -> torch.Tensor:
+        """Logits of hidden states, soft-capped, in the model's type."""
+        logits = module_linear(self.lm_head, hidden)
         if self.config.logit_softcap != 0:
             logits = self.config.logit_softcap * torch.tanh(logits / self.config.logit_softcap)
-        return CausalLMOutput(logits=logits.float(), past_key_values=cache)
+        return logits
+
+    def loss(self, input_ids: torch.Tensor, labels: torch.Tensor | None = None, *, teacher: TopLogits | None = None,
+             label_weight: float = 0.0, ignore_index: int = -100, reduction: str = "mean",
+             attention_mask=None) -> torch.Tensor:
+        """Training loss of a batch ``input_ids`` [B, T], differentiable in the model's parameters.
+
+        ``labels`` [B, T] are the token ids that the sequences hold (usually
+        ``input_ids`` itself): the logits of position t are scored against
+        labels[:, t + 1], and the last position counts for nothing.  Without a
+        ``teacher`` this is their cross-entropy.  With one (``top_logits`` of
+        another model on the same ``input_ids``) it is the distillation loss
+        of every position, ``label_weight`` of it the cross-entropy; labels
+        with ``ignore_index`` leave their position out of both.  The logits
+        stay in the model's type (``losses.py``)."""
+        if labels is None and teacher is None:
+            raise ValueError("loss needs labels, a teacher, or both")
+        if labels is not None and labels.shape != input_ids.shape:
+            raise ValueError(f"labels must have the shape of input_ids {tuple(input_ids.shape)}, "
+                             f"got {tuple(labels.shape)}")
+        hidden = self.transformer(input_ids=input_ids, attention_mask=attention_mask).last_hidden_state
+        targets = None
+        if labels is not None:
+            targets = torch.cat([labels[:, 1:], labels.new_full((labels.shape[0], 1), ignore_index)], dim=1)
+        logits = self._head(hidden)
+        if teacher is None:
+            return cross_entropy(logits, targets, ignore_index=ignore_index, reduction=reduction)
+        return distillation_loss(logits, teacher, targets, label_weight=label_weight, ignore_index=ignore_index,
+                                 reduction=reduction)
+
+    @torch.no_grad()
+    def top_logits(self, input_ids: torch.Tensor, k: int, *, temperature: float = 1.0) -> TopLogits:
+        """The model's ``k`` largest logits at every position of ``input_ids``
+        [B, T], as the teacher of another model's :meth:`loss`."""
+        return top_logits(self._head(self.transformer(input_ids=input_ids).last_hidden_state), k,
+                          temperature=temperature)
 
     @torch.no_grad()
     def generate_greedy(self, input_ids: torch.Tensor, max_new_tokens: int,
@@ -596,6 +637,56 @@ class RWKV7BackboneForCausalLM(nn.Module):
             logits = self(input_ids=tok[:, None], past_key_values=cache, use_cache=True,
                           cache_position=pos, logits_to_keep=1).logits[:, -1]
         return tokens
+
+    @torch.no_grad()
+    def generate_sampled(self, input_ids: torch.Tensor, max_new_tokens: int, *, temperature=1.0, top_k=0, top_p=1.0,
+                         min_p=0.0, uniforms: torch.Tensor | None = None, generator: torch.Generator | None = None,
+                         return_logprobs: bool = False,
+                         cache: StatesDictCache | None = None):
+        """:meth:`generate_greedy` with every token drawn by
+        ``logits.sample_tokens`` under ``temperature``, ``top_k``, ``top_p``
+        and ``min_p`` (numbers, or tensors [B]: one setting per sequence).
+        ``uniforms`` [B, max_new_tokens] in [0, 1) decide the draws; without
+        them they come from ``generator`` (torch's own when None).  Returns
+        int64 [B, max_new_tokens], with ``return_logprobs`` also the float32
+        log-probability of every token under what it was drawn from."""
+        B, T = input_ids.shape
+        cache = StatesDictCache() if cache is None else cache
+        u = _uniforms(uniforms, input_ids, max_new_tokens, generator)
+        logits = self(input_ids=input_ids, past_key_values=cache, use_cache=True,
+                      cache_position=torch.arange(T, device=input_ids.device), logits_to_keep=1).logits[:, -1]
+
+        def step(tok, s):
+            return self(input_ids=tok[:, None], past_key_values=cache, use_cache=True,
+                        cache_position=torch.tensor([T + s], device=input_ids.device), logits_to_keep=1).logits[:, -1]
+
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        return _sample_loop(logits, step, u, settings, return_logprobs)
+
+
+def _uniforms(uniforms, input_ids, n, generator):
+    """The uniform numbers of a generation, step by step: [n, B] float32."""
+    B = input_ids.shape[0]
+    if uniforms is None:
+        return torch.rand(n, B, generator=generator, device=input_ids.device)
+    if uniforms.shape != (B, n):
+        raise ValueError(f"uniforms must be [{B}, {n}] (batch, max_new_tokens), got {tuple(uniforms.shape)}")
+    return uniforms.t().to(device=input_ids.device, dtype=torch.float32).contiguous()
+
+
+def _sample_loop(logits, step, uniforms, settings, return_logprobs):
+    """Draws one token per row of uniforms [n, B] from the logits that
+    ``step(tokens, s)`` gives, the first from ``logits``."""
+    n, B = uniforms.shape
+    tokens = torch.empty(B, n, dtype=torch.long, device=uniforms.device)
+    logprobs = torch.empty(B, n, dtype=torch.float32, device=uniforms.device)
+    for s in range(n):
+        tok, lp = sample_tokens(logits, uniforms[s], **settings, return_logprobs=True)
+        tokens[:, s] = tok
+        logprobs[:, s] = lp
+        if s + 1 < n:
+            logits = step(tok, s)
+    return (tokens, logprobs) if return_logprobs else tokens
 
 
 class DecodeGraph:
@@ -740,6 +831,18 @@ class DecodeGraph:
                 break
             logits = self.step(tok)
         return tokens
+
+    @torch.no_grad()
+    def generate_sampled(self, input_ids: torch.Tensor, max_new_tokens: int, *, temperature=1.0, top_k=0, top_p=1.0,
+                         min_p=0.0, uniforms: torch.Tensor | None = None, generator: torch.Generator | None = None,
+                         return_logprobs: bool = False):
+        """``RWKV7BackboneForCausalLM.generate_sampled`` through this runner."""
+        B, T = input_ids.shape
+        u = _uniforms(uniforms, input_ids, max_new_tokens, generator)
+        logits = self.model(input_ids=input_ids, past_key_values=self.cache, use_cache=True,
+                            cache_position=torch.arange(T, device=input_ids.device), logits_to_keep=1).logits[:, -1]
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        return _sample_loop(logits, lambda tok, s: self.step(tok), u, settings, return_logprobs)
 
 
 @torch.no_grad()

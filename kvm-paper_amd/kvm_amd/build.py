@@ -9,16 +9,18 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG.parent / "csrc"
 OUT = PKG / "libkvm_amd.so"
 SOURCES = ["kvm_api.hip", "kvm_update.hip", "kvm_chain.hip", "kvm_decode.hip", "kvm_attn.hip", "kvm_attn_bwd.hip",
-           "kvm_state_bwd.hip", "kvm_prefix.hip", "kvm_gemm.hip", "kvm_block.hip"]
+           "kvm_state_bwd.hip", "kvm_prefix.hip", "kvm_gemm.hip", "kvm_block.hip", "kvm_loss.hip", "kvm_sample.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
-    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     # Keep the compiler from forming packed fp32 instructions.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
@@ -59,10 +61,16 @@ def build_ops(verbose: bool = False) -> Path:
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile every HIP source into one shared library, then the torch
-    operator library over it (always rebuilds)."""
+    """Compile every HIP source (side by side) into one shared library, then
+    the torch operator library over it (always rebuilds)."""
     tmp = OUT.with_suffix(".so.tmp")
-    _run([HIPCC, *FLAGS, "-o", str(tmp), *[str(CSRC / s) for s in SOURCES]], verbose)
+    with tempfile.TemporaryDirectory() as objs, ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        objects = [str(Path(objs) / (s + ".o")) for s in SOURCES]
+        jobs = [pool.submit(_run, [HIPCC, *FLAGS, "-c", "-o", o, str(CSRC / s)], verbose)
+                for s, o in zip(SOURCES, objects)]
+        for j in jobs:
+            j.result()
+        _run([HIPCC, "--offload-arch=gfx950", "-fPIC", "-shared", "-o", str(tmp), *objects], verbose)
     os.replace(tmp, OUT)
     build_ops(verbose)
     return OUT
