@@ -23,9 +23,9 @@
 // sum of exponentials, gradient; a forward that needs a gradient therefore
 // moves every logit once in and once out, and the backward has nothing left
 // to do but a factor.  The teacher's tokens are marked in a bitmap in LDS (one
-// bit per token, laid out as the chunks are: one LDS read per chunk), so that
-// the passes over the row skip them; their gradient is written after the
-// others' by the K threads that hold them.
+// bit per token, laid out as the chunks are: one LDS read per chunk) and hidden
+// in the registers, so that the passes are those of a plain softmax; their
+// gradient is written after the others' by the K threads that hold them.
 //
 // Sums and statistics are fp32, differences of logarithms of single tokens
 // fp64 (they cancel where student and teacher agree).  The gradient is rounded
@@ -62,7 +62,7 @@ __device__ __forceinline__ double log2_of(double ref, float s) {
 __device__ __forceinline__ float reference(float m) { return m == kNegInf ? 0.f : m; }
 
 template <int DT, int T, int NV, bool TEACHER>
-__global__ __launch_bounds__(T) void k_head_loss(kvm_head_loss_desc P) {
+__global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_head_loss(kvm_head_loss_desc P) {
   using R = Row<DT, T, NV>;
   using raw = typename R::raw;
   constexpr int N = R::N, W = T / kWave;
@@ -145,17 +145,30 @@ __global__ __launch_bounds__(T) void k_head_loss(kvm_head_loss_desc P) {
     }
     __syncthreads();
   }
-  // Bits of a chunk's tokens that the teacher names.
+  // Bits of a chunk's tokens that the teacher names.  In registers those
+  // tokens are hidden once; a row that is read again hides them on every pass.
   auto named = [&](int i0, int n) -> uint32_t {
-    if constexpr (!TEACHER) return 0;
     if (n == 0) return 0;
     const int pos = x.shifted(i0);
     return bits[pos >> 5] >> (pos & 31);
   };
-  x.each([&](const float (&v)[N], int i0, int n) {
-    const uint32_t nm = named(i0, n);
+  if constexpr (TEACHER) x.hide(named);
+  auto others = [&](auto &&f) {
+    x.each([&](const float (&v)[N], int i0, int n) {
+      if constexpr (TEACHER && NV == 0) {
+        const uint32_t nm = named(i0, n);
+        float u[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) m_o = fmaxf(m_o, TEACHER && (nm >> i & 1) ? kNegInf : v[i]);
+        for (int i = 0; i < N; ++i) u[i] = nm >> i & 1 ? kNegInf : v[i];
+        f(u, i0, n);
+      } else {
+        f(v, i0, n);
+      }
+    });
+  };
+  others([&](const float (&v)[N], int, int) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) m_o = fmaxf(m_o, v[i]);
   });
   m_o = wave_max(m_o);
   if constexpr (TEACHER) {
@@ -168,11 +181,10 @@ __global__ __launch_bounds__(T) void k_head_loss(kvm_head_loss_desc P) {
     red_a[wave][2] = m_o;
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    m_t = fmaxf(m_t, red_a[w][0]);
-    m_x = fmaxf(m_x, red_a[w][1]);
-    m_o = fmaxf(m_o, red_a[w][2]);
+  m_o = part_max<W>(&red_a[0][2], 3);
+  if constexpr (TEACHER) {
+    m_t = part_max<W>(&red_a[0][0], 3);
+    m_x = part_max<W>(&red_a[0][1], 3);
   }
   const bool dups = TEACHER && dup;
   // ---- sums of exponentials.  Every logarithm below is relative to the
@@ -185,14 +197,20 @@ __global__ __launch_bounds__(T) void k_head_loss(kvm_head_loss_desc P) {
   const double rest2 = TEACHER && P.t_rest ? double(P.t_rest[row]) * 1.4426950408889634 : -__builtin_inf();
   double top2 = fmax(double(m_t) * c, rest2);
   if (top2 == -__builtin_inf()) top2 = 0.0;
+  // exp(v - m_o) from e = exp((v - m_o) / T): a power of it for the usual whole T.
+  const int whole = tau == 2.f ? 2 : tau == 4.f ? 4 : 0;
+  auto at_one = [&](float v, float e) -> float {
+    if (whole == 0) return exp2_fast((v - m_o) * kLog2e);
+    const float e2 = e * e;
+    return whole == 2 ? e2 : e2 * e2;
+  };
   float z_o = 0.f, z_o1 = 0.f, z_t = 0.f, z_x = 0.f, z_x1 = 0.f;
-  x.each([&](const float (&v)[N], int i0, int n) {
-    const uint32_t nm = named(i0, n);
+  others([&](const float (&v)[N], int, int) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float u = TEACHER && (nm >> i & 1) ? kNegInf : v[i];
-      z_o += exp2_fast((u - m_o) * c);
-      if (two) z_o1 += exp2_fast((u - m_o) * kLog2e);
+      const float e = exp2_fast((v[i] - m_o) * c);
+      z_o += e;
+      if (two) z_o1 += at_one(v[i], e);
     }
   });
   // The lowest of the entries that name a token stands for it in the student's sums.
@@ -227,14 +245,12 @@ __global__ __launch_bounds__(T) void k_head_loss(kvm_head_loss_desc P) {
     red_b[wave][4] = z_x1;
   }
   __syncthreads();
-  z_o = z_o1 = z_t = z_x = z_x1 = 0.f;
-#pragma unroll
-  for (int w = 0; w < W; ++w) {
-    z_o += red_b[w][0];
-    z_o1 += red_b[w][1];
-    z_t += red_b[w][2];
-    z_x += red_b[w][3];
-    z_x1 += red_b[w][4];
+  z_o = part_add<W>(&red_b[0][0], 5);
+  if constexpr (TEACHER) {
+    z_o1 = part_add<W>(&red_b[0][1], 5);
+    z_t = part_add<W>(&red_b[0][2], 5);
+    z_x = part_add<W>(&red_b[0][3], 5);
+    z_x1 = part_add<W>(&red_b[0][4], 5);
   }
   // ---- logarithms of the row's sums (log2 units, relative to m)
   const double off_o = double(m_o) - m, off_x = double(m_x) - m;
@@ -291,8 +307,9 @@ __global__ __launch_bounds__(T) void k_head_loss(kvm_head_loss_desc P) {
   }
   if (hard) (two ? f1 : f) += w_hard * exp2_fast(float(off_o * (two ? kLog2e : c) - lse21));
   auto other = [&](float v) -> float {
-    float g = f * exp2_fast((v - m_o) * c);
-    if (two) g += f1 * exp2_fast((v - m_o) * kLog2e);
+    const float e = exp2_fast((v - m_o) * c);
+    float g = f * e;
+    if (two) g += f1 * at_one(v, e);
     return g;
   };
   x.each([&](const float (&v)[N], int i0, int n) {

@@ -87,6 +87,23 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
 }
 
+// The same over the W <= 16 partial results of a workgroup's waves, part[0],
+// part[stride], ...: one LDS read per lane, the same value in every lane.
+template <int W>
+__device__ __forceinline__ float part_add(const float *part, int stride = 1) {
+  const int l = threadIdx.x & 15;
+  return group_sum<16>(l < W ? part[l * stride] : 0.f);
+}
+template <int W>
+__device__ __forceinline__ float part_max(const float *part, int stride = 1) {
+  const int l = threadIdx.x & 15;
+  float v = l < W ? part[l * stride] : kNegInf;
+  v = fmaxf(v, dpp<kDppRowRor8>(v));
+  v = fmaxf(v, dpp<kDppRowRor4>(v));
+  v = fmaxf(v, dpp<kDppQuadXor2>(v));
+  return fmaxf(v, dpp<kDppQuadXor1>(v));
+}
+
 // A row of V values in the registers of a workgroup of T threads, NV chunks
 // per thread (NV = 0: read again on every pass; for rows that do not fit).
 template <int DT, int T, int NV>
@@ -137,6 +154,30 @@ struct Row {
   // Position of value idx in an array that is laid out as the chunks are:
   // the first value of every chunk lies at a multiple of N.
   __device__ __forceinline__ int shifted(int idx) const { return idx + (head ? N - head : 0); }
+
+  // Replaces the values that f(first, n) names (bit i: value first + i) by
+  // -infinity, in the registers; rows that are read again keep them.
+  template <class F>
+  __device__ __forceinline__ void hide(F &&f) {
+    const int t = threadIdx.x;
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (j * T < nfull) {
+          const int c = j * T + t;
+          const uint32_t bits = c < nfull ? f(head + c * N, N) : 0;
+          if (bits & ((1u << N) - 1)) {
+            float x[N];
+            E::unpack(v[j], x);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = bits >> i & 1 ? kNegInf : x[i];
+            v[j] = E::pack(x);
+          }
+        }
+      }
+      if (edge_idx >= 0 && (f(edge_idx, 1) & 1)) edge = kNegInf;
+    }
+  }
 
   // f(x, first, n): n values x[0..n) with indices first, first + 1, ...  n is
   // N, or 1 (a value outside the chunks), or 0 (none); the values past n are

@@ -17,17 +17,21 @@
 // passes floor(u C).  A row is never sorted: all that is needed is to find the
 // token at a given running sum (or rank), "locating" it.
 //
+// The first tokens of the order come cheaply: the k-th largest of the threads'
+// own maxima is a lower bound of the k-th largest logit that few other logits
+// pass (T ln(1 / (1 - k/T)) of them for T threads and logits in no particular
+// order); those that do are collected and ranked by counting, each against
+// each.  That is all that the top logits and a small top-k need.  Without one,
+// sampling adds up the weights of the whole row, and is done where the tokens
+// so ranked hold what top-p asks for and the draw falls on one of them, as it
+// does unless a distribution is rather flat.
+//
 // Locating, in general: a histogram of weights (or counts) over 2048 bins that
 // are linear in (x_0 - x) / T up to the 43 ln 2 past which weights are zero; a
 // prefix sum over it names the bin; the bin's tokens (about 50 for logits with
-// a spread of a few nats) are collected and ranked by counting, each against
-// each.  A bin with more than 1024 tokens is cut again by their bit patterns
-// until it has fewer, or holds one value only, whose tokens rank by index.
-//
-// Locating, for k up to half the workgroup: the k-th largest of the threads'
-// own maxima is a lower bound of the k-th largest logit that few other logits
-// pass (T ln(1 / (1 - k/T)) for T threads and logits in no particular order);
-// those that do are collected and ranked by counting.
+// a spread of a few nats) are collected and ranked by counting.  A bin with
+// more than 1024 tokens is cut again by their bit patterns until it has fewer,
+// or holds one value only, whose tokens rank by index.
 //
 // One workgroup per row.  The top logits hold the row in registers; sampling
 // reads it again on every pass, from the caches, in loops that are not unrolled
@@ -42,7 +46,6 @@ typedef unsigned long long u64;
 
 constexpr int kBins = 2048;
 constexpr int kCand = 1024;        // tokens that are ranked by counting
-constexpr int kSampleThreads = 1024;
 constexpr int kMaxTop = 512;       // K of the top logits
 constexpr double kUnit = 4398046511104.0;  // 2^42
 
@@ -59,41 +62,47 @@ __device__ __forceinline__ u64 rank_of(uint32_t key, int idx) { return u64(key) 
 __device__ __forceinline__ int index_of(u64 rank) { return int(0xffffffffu - uint32_t(rank)); }
 __device__ __forceinline__ uint32_t key_part(u64 rank) { return uint32_t(rank >> 32); }
 
-// 2^y for y <= 0 in fp64, relative error below 2^-50: 2^n times the Taylor
-// series of 2^f = exp(f ln 2), |f| <= 1/2, to the twelfth power.
-// No contraction: a token's weight is the same wherever it is computed.
-__device__ __forceinline__ double exp2_wide(double y) {
+// 2^(i / 64) for the weights' exponentials: the Taylor series of exp(f ln 2).
+constexpr int kTable = 64;
+__device__ __forceinline__ double exp2_fraction(int i) {
 #pragma clang fp contract(off)
-  const double n = rint(y), f = (y - n) * 0.6931471805599453;
-  double p = 1.0 / 479001600.0;
-  p = __builtin_fma(p, f, 1.0 / 39916800.0);
-  p = __builtin_fma(p, f, 1.0 / 3628800.0);
-  p = __builtin_fma(p, f, 1.0 / 362880.0);
-  p = __builtin_fma(p, f, 1.0 / 40320.0);
-  p = __builtin_fma(p, f, 1.0 / 5040.0);
-  p = __builtin_fma(p, f, 1.0 / 720.0);
-  p = __builtin_fma(p, f, 1.0 / 120.0);
-  p = __builtin_fma(p, f, 1.0 / 24.0);
-  p = __builtin_fma(p, f, 1.0 / 6.0);
-  p = __builtin_fma(p, f, 0.5);
-  p = __builtin_fma(p, f, 1.0);
-  p = __builtin_fma(p, f, 1.0);
-  return ldexp(p, int(n));
+  const double f = double(i) * (0.6931471805599453 / kTable);
+  double p = 1.0, term = 1.0;
+  for (int k = 1; k <= 20; ++k) {
+    term *= f / double(k);
+    p += term;
+  }
+  return p;
 }
 
 // Weights and bins of a row at one temperature.
 struct Weights {
-  float best;      // x_0
-  double log2_per; // log2(e) / T
-  float bins_per;  // bins per unit of logit
+  float best;          // x_0
+  double per;          // 64 log2(e) / T
+  float bins_per;      // bins per unit of logit
+  const double *table; // 2^(i / 64)
+  // floor(2^42 exp((x - best) / T) + 1/2): 2^(n / 64) from the table and the
+  // exponent, the rest by the Taylor series to the fifth power (|f| <= ln 2 /
+  // 128: off by less than 2^-54).  No contraction: a token's weight is the
+  // same wherever it is computed.
   __device__ __forceinline__ u64 operator()(float x) const {
 #pragma clang fp contract(off)
-    if (x == best) return u64(kUnit);
-    const double y = (double(x) - double(best)) * log2_per;
-    if (!(y >= -43.0)) return 0;
-    // 2^42 e + 1/2 is below 2^43: adding 2^52 to the product rounds it to a
-    // whole number in the low bits.
-    return __builtin_bit_cast(u64, __builtin_fma(exp2_wide(y), kUnit, 4503599627370496.0)) & 0xfffffffffffffull;
+    double y = (double(x) - double(best)) * per;
+    if (x == best) y = 0.0;  // infinity less itself
+    const bool some = y >= -43.0 * kTable;
+    if (!some) y = 0.0;
+    const double n = rint(y), f = (y - n) * (0.6931471805599453 / kTable);
+    double p = 1.0 / 120.0;
+    p = __builtin_fma(p, f, 1.0 / 24.0);
+    p = __builtin_fma(p, f, 1.0 / 6.0);
+    p = __builtin_fma(p, f, 0.5);
+    p = __builtin_fma(p, f, 1.0);
+    p = __builtin_fma(p, f, 1.0);
+    const int k = int(n);
+    const double unit = __builtin_bit_cast(double, u64(1023 + 42 + (k >> 6)) << 52);  // 2^42 times the whole part
+    // Below 2^43: adding 2^52 rounds to a whole number in the low bits.
+    const double w = __builtin_fma(table[k & (kTable - 1)] * p, unit, 4503599627370496.0);
+    return some ? __builtin_bit_cast(u64, w) & 0xfffffffffffffull : 0;
   }
   __device__ __forceinline__ int bin(float x) const {
     const float d = x == best ? 0.f : best - x;
@@ -114,7 +123,8 @@ struct Shared {
   u64 base;        // weight (or count) before the located bin
   u64 found;       // the located token (its rank_of)
   u64 found_end;   // running sum including it
-  uint32_t bound;
+  int above;       // of a bound: thread maxima before its bin
+  double table[kTable];
 };
 
 template <int T>
@@ -123,9 +133,7 @@ __device__ __forceinline__ float block_max(float v, float *red) {
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < T / kWave; ++w) v = fmaxf(v, red[w]);
-  return v;
+  return part_max<T / kWave>(red);
 }
 template <int T>
 __device__ __forceinline__ int block_min(int v, int *red) {
@@ -200,47 +208,102 @@ __device__ __forceinline__ int collect_above(const R &x, uint32_t bound, Shared 
   return sh.count;
 }
 
-// A lower bound of the k-th largest key of the row: (about) the k-th largest
-// of the threads' maxima, found by bisection in the first wave.  T >= k.
-template <int T, class R>
+// A lower bound of the k-th largest key of the row: one of the threads' maxima
+// that k of them or a few more reach, from a histogram of the maxima over 256
+// bins, twice.  Where fewer than k threads hold a number, -infinity's key.
+template <int T>
 __device__ __forceinline__ uint32_t bound_of(float thread_max, int k, Shared &sh) {
-  uint32_t *keys = reinterpret_cast<uint32_t *>(sh.fine);
+  constexpr int kCuts = 256;
+  uint32_t *hist = reinterpret_cast<uint32_t *>(sh.fine);
   const int t = threadIdx.x;
-  keys[t] = key_of(thread_max);
-  __syncthreads();
-  if (t < kWave) {
-    constexpr int M = T / kWave;
-    uint32_t mine[M], lo = 0xffffffffu, hi = 0;
-#pragma unroll
-    for (int i = 0; i < M; ++i) {
-      mine[i] = keys[i * kWave + t];
-      lo = min(lo, mine[i]);
-      hi = max(hi, mine[i]);
+  const uint32_t mine = key_of(thread_max), none = 0x007fffffu;  // -infinity's
+  bool in = mine != none;
+  int above = 0;
+  uint32_t bound = none;
+#pragma unroll 1
+  for (int level = 0; level < 2; ++level) {
+    __syncthreads();
+    for (int i = t; i < kCuts; i += T) hist[i] = 0;
+    if (t == 0) {
+      sh.kmin = 0xffffffffu;
+      sh.kmax = 0;
+      sh.bin = -1;
     }
+    __syncthreads();
+    uint32_t lo = in ? mine : 0xffffffffu, hi = in ? mine : 0;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
       lo = min(lo, uint32_t(__shfl_xor(int(lo), o)));
       hi = max(hi, uint32_t(__shfl_xor(int(hi), o)));
     }
-    // Invariant: at least k keys are >= lo.  An interval that passes a few
-    // more than k keys is good enough.
-    const int enough = k + k / 8;
-    while (hi - lo > 1) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      int c = 0;
+    if ((t & 63) == 0) {
+      atomicMin(&sh.kmin, lo);
+      atomicMax(&sh.kmax, hi);
+    }
+    __syncthreads();
+    lo = sh.kmin;
+    hi = sh.kmax;
+    const float per = float(kCuts) / (float(hi - lo) + 1.f);
+    const int cut = in ? min(int(float(hi - mine) * per), kCuts - 1) : kCuts;
+    if (in) atomicAdd(&hist[cut], 1u);
+    __syncthreads();
+    if (t < kWave) {
+      uint32_t q[kCuts / kWave], own = 0;
 #pragma unroll
-      for (int i = 0; i < M; ++i) c += __popcll(__ballot(mine[i] >= mid));
-      if (c >= k) {
-        lo = mid;
-        if (c <= enough) break;
-      } else {
-        hi = mid;
+      for (int i = 0; i < kCuts / kWave; ++i) own += q[i] = hist[t * (kCuts / kWave) + i];
+      uint32_t s = own;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const uint32_t up = __shfl_up(s, o);
+        if (t >= o) s += up;
+      }
+      s += above - own;
+#pragma unroll
+      for (int i = 0; i < kCuts / kWave; ++i) {
+        if (int(s) < k && int(s + q[i]) >= k) {
+          sh.bin = t * (kCuts / kWave) + i;
+          sh.above = int(s);
+          sh.count = int(s + q[i]);
+        }
+        s += q[i];
       }
     }
-    if (t == 0) sh.bound = lo;
+    __syncthreads();
+    const int bin = sh.bin, reach = sh.count;
+    if (bin < 0) return none;  // fewer than k numbers
+    above = sh.above;
+    // the smallest maximum of that bin
+    uint32_t least = cut == bin ? mine : 0xffffffffu;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) least = min(least, uint32_t(__shfl_xor(int(least), o)));
+    if (t == 0) sh.kmin = 0xffffffffu;  // read by all before the last barrier
+    __syncthreads();
+    if ((t & 63) == 0) atomicMin(&sh.kmin, least);
+    __syncthreads();
+    bound = sh.kmin;
+    if (reach <= k + k / 4 + 8) break;
+    in = cut == bin;
   }
-  __syncthreads();
-  return sh.bound;
+  return bound;
+}
+
+// f(i, token, rank) for the cnt tokens of the list, rank = how many of them
+// come before it, once per token (by one lane).  A token is compared by as
+// many lanes as there are to spare.
+template <int T, class F>
+__device__ __forceinline__ void ranked(int cnt, const Shared &sh, F &&f) {
+  const int t = threadIdx.x;
+  int lanes = 1;
+  while (lanes < 16 && 2 * lanes * cnt <= T) lanes *= 2;
+  const int part = t & (lanes - 1);
+  for (int i0 = 0; i0 < cnt; i0 += T / lanes) {
+    const int i = i0 + t / lanes;
+    const u64 me = sh.cand[min(i, cnt - 1)];
+    int r = 0;
+    for (int j = part; j < cnt; j += lanes) r += sh.cand[j] > me;
+    for (int o = lanes / 2; o >= 1; o >>= 1) r += __shfl_xor(r, o);
+    if (part == 0 && i < cnt) f(i, me, r);
+  }
 }
 
 // The token at running sum `target` (before <= target < before + its own) in
@@ -285,11 +348,11 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         if (i < n) {
+          if (wt.bin(v[i]) != bin) continue;
           const uint32_t k = key_of(v[i]);
-          const float xv = value_of(k);
-          bool hit = k >= lo && k <= hi && wt.bin(xv) == bin;
+          bool hit = k >= lo && k <= hi;
           if (hit && !first) hit = int(u64(f_hi - k) * kBins / (u64(f_span) + 1)) == f_bin;
-          if (hit && in(xv, i0 + i)) {
+          if (hit && in(v[i], i0 + i)) {
             a = min(a, k);
             b = max(b, k);
             const int at = atomicAdd(&sh.count, 1);
@@ -309,11 +372,17 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
     if (cnt <= kCand) {
       for (int i = t; i < cnt; i += T) sh.cw[i] = COUNT ? 1 : wt(value_of(key_part(sh.cand[i])));
       __syncthreads();
-      for (int i = t; i < cnt; i += T) {
+      int lanes = 1;
+      while (lanes < 16 && 2 * lanes * cnt <= T) lanes *= 2;
+      const int part = t & (lanes - 1);
+      for (int i0 = 0; i0 < cnt; i0 += T / lanes) {
+        const int i = min(i0 + t / lanes, cnt - 1);
         const u64 me = sh.cand[i];
-        u64 before = base;
-        for (int j = 0; j < cnt; ++j)
+        u64 before = 0;
+        for (int j = part; j < cnt; j += lanes)
           if (sh.cand[j] > me) before += sh.cw[j];
+        for (int o = lanes / 2; o >= 1; o >>= 1) before += __shfl_xor(before, o);
+        before += base;
         if (target >= before && target < before + sh.cw[i]) {
           sh.found = me;
           sh.found_end = before + sh.cw[i];
@@ -357,10 +426,10 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
     x.each([&](const float (&v)[N], int i0, int n) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
+        if (i >= n || wt.bin(v[i]) != bin) continue;
         const uint32_t k = key_of(v[i]);
-        const float xv = value_of(k);
-        if (i < n && k >= lo && k <= hi && wt.bin(xv) == bin && in(xv, i0 + i))
-          atomicAdd(&sh.fine[int(u64(f_hi - k) * kBins / (u64(f_span) + 1))], COUNT ? 1 : wt(xv));
+        if (k >= lo && k <= hi && in(v[i], i0 + i))
+          atomicAdd(&sh.fine[int(u64(f_hi - k) * kBins / (u64(f_span) + 1))], COUNT ? 1 : wt(v[i]));
       }
     });
     __syncthreads();
@@ -429,9 +498,8 @@ __device__ __forceinline__ u64 target_of(float u, u64 c) {
   return at >= double(last) ? last : u64(at);
 }
 
-template <int DT>
-__global__ __launch_bounds__(kSampleThreads) void k_sample(kvm_sample_desc P) {
-  constexpr int T = kSampleThreads;
+template <int DT, int T>
+__global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_sample(kvm_sample_desc P) {
   using R = Row<DT, T, 0>;
   constexpr int N = R::N;
   __shared__ Shared sh;
@@ -446,6 +514,7 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(kvm_sample_desc P) {
   min_p = min_p > 0.f ? min_p : 0.f;
   const int top_k = P.top_k ? P.top_k[row] : int(P.top_k_all);
   const float u = P.uniforms[row];
+  if (t < kTable) sh.table[t] = exp2_fraction(t);
 
   float mine = kNegInf;
   x.each([&](const float (&v)[N], int, int) {
@@ -474,9 +543,10 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(kvm_sample_desc P) {
   }
   Weights wt;
   wt.best = best;
-  wt.log2_per = 1.4426950408889634 / double(temp);
+  wt.per = kTable * 1.4426950408889634 / double(temp);
   // 43 octaves of weight fill the bins
   wt.bins_per = float(double(kBins) / (43.0 * 0.6931471805599453 * double(temp)));
+  wt.table = sh.table;
   const double least = double(min_p) * kUnit;
   auto write = [&](u64 rank, u64 c) {  // one thread: the token and ln(w / C)
     const float xv = value_of(key_part(rank));
@@ -484,35 +554,59 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(kvm_sample_desc P) {
     answer(index_of(rank), float(d - log(double(c) / kUnit)));
   };
 
-  if (top_k > 0 && top_k <= T / 2 && top_k < V) {
-    const uint32_t bound = bound_of<T, R>(mine, top_k, sh);
-    const int cnt = collect_above<T>(x, bound, sh);
-    if (cnt <= kCand) {
-      const int k = min(top_k, cnt);
-      u64 *sorted = sh.hist;
-      for (int i = t; i < cnt; i += T) {
-        const u64 me = sh.cand[i];
-        int r = 0;
-        for (int j = 0; j < cnt; ++j) r += sh.cand[j] > me;
-        if (r < k) sorted[r] = me;
+  // The first tokens of the order.
+  const bool some = top_k > 0 && top_k < V;  // top-k drops tokens
+  const bool few = some && top_k <= T / 2;
+  const uint32_t bound = bound_of<T>(mine, few ? top_k : T / 4, sh);
+  const int cnt = collect_above<T>(x, bound, sh);
+  const bool covers = few || cnt == V;  // no token past the list is kept
+  if (cnt <= min(kCand, T) && (covers || !some)) {
+    u64 *sorted = sh.hist;
+    ranked<T>(cnt, sh, [&](int, u64 me, int r) { sorted[r] = me; });
+    u64 z = 0, strong = 0;
+    if (!covers) {  // the weight of the whole row
+      x.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const u64 w = wt(v[i]);
+          z += w;
+          if (min_p > 0.f && double(w) >= least) strong += w;
+        }
+      });
+      z = block_add<T>(z, sh.scan);
+      if (min_p > 0.f) strong = block_add<T>(strong, sh.scan);
+    }
+    __syncthreads();
+    const int k = some ? min(top_k, cnt) : cnt;
+    const u64 me = t < k ? sorted[t] : 0;  // one token per thread
+    const u64 w = t < k ? wt(value_of(key_part(me))) : 0;
+    u64 sum;
+    const u64 before = block_scan<T>(w, sh.scan, &sum);
+    if (covers) z = sum;
+    const double end = double(top_p) * double(z);
+    // The weight that is kept: inside the list as a sum of it, past it as one of the row.
+    const bool keep = t == 0 || (double(before) < end && double(w) >= least);
+    const u64 c_list = block_add<T>(keep ? w : 0, sh.scan);
+    u64 c = c_list;
+    bool known = true;
+    if (!covers) {
+      const bool p_in = top_p < 1.f && double(sum) >= end;
+      const bool m_in = min_p > 0.f && strong < sum;
+      if (!p_in && !m_in) {
+        known = top_p >= 1.f;
+        c = min_p > 0.f ? strong : z;
       }
-      __syncthreads();
-      const u64 me = t < k ? sorted[t] : 0;  // k <= T / 2: one token per thread
-      const u64 w = t < k ? wt(value_of(key_part(me))) : 0;
-      u64 z;
-      const u64 before = block_scan<T>(w, sh.scan, &z);
-      const bool keep = t == 0 || (double(before) < double(top_p) * double(z) && double(w) >= least);
-      const u64 c = block_add<T>(keep ? w : 0, sh.scan);
-      const u64 at = target_of(u, c);
+    }
+    const u64 at = target_of(u, c);
+    if (known && at < sum) {
       if (at >= before && at < before + w) write(me, c);
       return;
     }
-    __syncthreads();
   }
   auto all = [](float, int) { return true; };
   u64 limit = 0;  // the last token that top-k keeps (0: it keeps all)
   u64 z;
-  if (top_k > 0 && top_k < V) {
+  if (some) {
     const u64 pre = build<T, true>(x, wt, sh, &z, 0.0, nullptr, all);
     if (u64(top_k) < z) {
       auto positive = [&](float v, int) { return wt(v) != 0; };
@@ -525,23 +619,25 @@ __global__ __launch_bounds__(kSampleThreads) void k_sample(kvm_sample_desc P) {
   const u64 pre = build<T, false>(x, wt, sh, &z, least, min_p > 0.f ? &strong : nullptr, kept);
   auto weighted = [&](float v, int i) { return kept(v, i) && wt(v) != 0; };
   u64 c = z;
-  if (top_p < 1.f) {
-    const double end = ceil(double(top_p) * double(z));
-    if (end >= 1.0) {
-      locate<T, false>(x, wt, u64(end) - 1, pre, sh, weighted);
-      c = sh.found_end;
+#pragma unroll 1
+  for (int step = top_p < 1.f ? 0 : 1; step < 2; ++step) {  // where top-p ends, then the draw
+    u64 target;
+    if (step == 0) {
+      const double end = ceil(double(top_p) * double(z));
+      target = end >= 1.0 ? u64(end) - 1 : 0;
     } else {
-      c = 0;
+      if (min_p > 0.f && strong < c) c = strong;
+      if (c < u64(kUnit)) c = u64(kUnit);  // the first token is always kept
+      target = target_of(u, c);
     }
+    locate<T, false>(x, wt, target, pre, sh, weighted);
+    if (step == 0) c = sh.found_end;
   }
-  if (min_p > 0.f && strong < c) c = strong;
-  if (c < u64(kUnit)) c = u64(kUnit);  // the first token is always kept
-  locate<T, false>(x, wt, target_of(u, c), pre, sh, weighted);
   if (t == 0) write(sh.found, c);
 }
 
 template <int DT, int T, int NV>
-__global__ __launch_bounds__(T) void k_top_logits(kvm_logits L, int K, float scale, void *values, int64_t *indices,
+__global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_top_logits(kvm_logits L, int K, float scale, void *values, int64_t *indices,
                                                   float *rest) {
   using R = Row<DT, T, NV>;
   using E = Elem<DT>;
@@ -558,15 +654,16 @@ __global__ __launch_bounds__(T) void k_top_logits(kvm_logits L, int K, float sca
     for (int i = 0; i < N; ++i) mine = fmaxf(mine, v[i]);
   });
   if (t == 0) s_next = 0;
-  const uint32_t bound = bound_of<T, R>(mine, K, sh);
+  const uint32_t bound = bound_of<T>(mine, K, sh);
   int cnt = collect_above<T>(x, bound, sh);
   u64 more_ties = 0;  // tokens of the K-th value behind it that are not in the list
   if (cnt > kCand) {
     // Many equal or clustered logits: the K-th token by rank, then exactly K are collected.
     Weights wt;  // one bin: the tokens are cut by their keys from the start
     wt.best = 0.f;
-    wt.log2_per = 0.0;
+    wt.per = 0.0;
     wt.bins_per = 0.f;
+    wt.table = sh.table;
     __syncthreads();
     for (int i = t; i < kBins; i += T) sh.hist[i] = i ? 0 : u64(V);
     auto all = [](float, int) { return true; };
@@ -598,17 +695,14 @@ __global__ __launch_bounds__(T) void k_top_logits(kvm_logits L, int K, float sca
     cnt = K;
   }
   u64 in_list = 0;
-  for (int i = t; i < cnt; i += T) {
-    const u64 me = sh.cand[i];
-    int r = 0;
-    for (int j = 0; j < cnt; ++j) r += sh.cand[j] > me;
+  ranked<T>(cnt, sh, [&](int, u64 me, int r) {
     if (r < K) {
       static_cast<typename E::raw *>(values)[int64_t(row) * K + r] = E::put(value_of(key_part(me)));
       indices[int64_t(row) * K + r] = index_of(me);
     }
     if (r == K - 1) s_last = me;
     if (r == K) s_next = me;
-  }
+  });
   if (!rest) return;
   __syncthreads();
   const u64 last = s_last, next = s_next;
@@ -639,11 +733,10 @@ __global__ __launch_bounds__(T) void k_top_logits(kvm_logits L, int K, float sca
   __syncthreads();
   if ((t & 63) == 0) sh.red[t >> 6] = z;
   __syncthreads();
-  if (t == 0) {
-    z = ties;  // each of them is the reference itself: m = vk, exp = 1
-    for (int w = 0; w < T / kWave; ++w) z += sh.red[w];
+  if (t < 16) {
+    z = ties + part_add<T / kWave>(sh.red);  // each of the ties is the reference itself: m = vk, exp = 1
     const double lse = m == kNegInf ? -__builtin_inf() : (double(ref) * scale + log2(double(z))) * 0.6931471805599453;
-    rest[row] = float(lse);
+    if (t == 0) rest[row] = float(lse);
   }
 }
 
@@ -667,13 +760,23 @@ struct TopLaunch {
 int64_t top_logits_max() { return kMaxTop; }
 
 hipError_t launch_sample(const kvm_sample_desc &P, hipStream_t stream) {
-  const dim3 grid(unsigned(P.logits.outer * P.logits.inner)), block(kSampleThreads);
-  if (P.logits.dtype == KVM_BF16)
-    hipLaunchKernelGGL(k_sample<KVM_BF16>, grid, block, 0, stream, P);
-  else if (P.logits.dtype == KVM_F16)
-    hipLaunchKernelGGL(k_sample<KVM_F16>, grid, block, 0, stream, P);
-  else
-    hipLaunchKernelGGL(k_sample<KVM_F32>, grid, block, 0, stream, P);
+  // Up to one row per compute unit: 1024 threads finish a row soonest; more
+  // rows: workgroups of 512, two of which share a compute unit.
+  const int64_t rows = P.logits.outer * P.logits.inner;
+  const dim3 grid{unsigned(rows)};
+#define KVM_SAMPLE(D)                                                                \
+  if (rows <= 256)                                                                   \
+    hipLaunchKernelGGL((k_sample<D, 1024>), grid, dim3(1024), 0, stream, P);         \
+  else                                                                               \
+    hipLaunchKernelGGL((k_sample<D, 512>), grid, dim3(512), 0, stream, P);
+  if (P.logits.dtype == KVM_BF16) {
+    KVM_SAMPLE(KVM_BF16)
+  } else if (P.logits.dtype == KVM_F16) {
+    KVM_SAMPLE(KVM_F16)
+  } else {
+    KVM_SAMPLE(KVM_F32)
+  }
+#undef KVM_SAMPLE
   return hipGetLastError();
 }
 

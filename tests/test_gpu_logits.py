@@ -92,6 +92,14 @@ def test_sample_settings(kw):
     _check_sample(_logits(8, 9001, torch.float32, 5), torch.rand(8, generator=_gen(6)), "settings", **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(top_k=550), dict(top_k=400, top_p=0.8), dict(top_p=0.97), dict(min_p=0.01),
+                                dict(top_p=0.9, min_p=0.02, temperature=3.0), dict(temperature=50.0)])
+@pytest.mark.parametrize("V,n", [(600, 4), (700, 300), (2500, 300)])
+def test_sample_short_rows_and_many_rows(V, n, kw):
+    """Rows that one list of tokens covers, and more rows than compute units."""
+    _check_sample(_logits(n, V, torch.bfloat16, V, 1.0), torch.rand(n, generator=_gen(V + n)), "short", **kw)
+
+
 def test_sample_settings_per_row():
     n = 24
     g = _gen(9)
