@@ -47,16 +47,21 @@ __device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// log2(z) of a sum z >= 1 or so, off by about 2e-7 whatever its size: the
+// fp32 logarithm and one Newton step on z 2^-l = 1.  -infinity for 0.
+__device__ __forceinline__ double log2_fine(float z) {
+  const float l = __log2f(z);
+  const float fix = __builtin_fmaf(z, exp2_fast(-l), -1.f) * kLog2e;
+  return z > 0.f ? double(l) + double(fix) : double(l);
+}
 // log2(2^a + 2^b) for doubles that may be -infinity.
 __device__ __forceinline__ double log2_add(double a, double b) {
   const double m = fmax(a, b);
   if (m == -__builtin_inf()) return m;
-  return m + double(__log2f(exp2_fast(float(a - m)) + exp2_fast(float(b - m))));
+  return m + log2_fine(exp2_fast(float(a - m)) + exp2_fast(float(b - m)));
 }
 // log2 of a sum s of 2^(v - ref): ref + log2(s), -infinity for an empty sum.
-__device__ __forceinline__ double log2_of(double ref, float s) {
-  return s > 0.f ? ref + log2(double(s)) : (s == 0.f ? -__builtin_inf() : double(s));
-}
+__device__ __forceinline__ double log2_of(double ref, float s) { return ref + log2_fine(s); }
 // The reference of a sum of exponentials: the maximum, or 0 where there is
 // none (every value -infinity), so that -infinity - reference stays -infinity.
 __device__ __forceinline__ float reference(float m) { return m == kNegInf ? 0.f : m; }
@@ -80,6 +85,16 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
   }
   int64_t label = P.labels ? P.labels[row] : 0;
   const bool ignored = P.labels && label == P.ignore_index;
+  // The teacher's first entries are asked for before the row: what depends on
+  // them (the bitmap, the student's logits there) need not wait for the row.
+  int64_t id_first = -1;
+  float tv_first = kNegInf;
+  if constexpr (TEACHER) {
+    if (t < K) {
+      id_first = P.t_indices[int64_t(row) * K + t];
+      tv_first = load_any(P.t_values, int64_t(row) * K + t, int(P.t_dtype));
+    }
+  }
   R x;
   x.open(logits_row<DT>(P.logits, row), V);
   if (ignored) {  // uniform: no loss, a gradient of zeros
@@ -125,11 +140,11 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
   float m_t = kNegInf, m_x = kNegInf, m_o = kNegInf;
   if constexpr (TEACHER) {
     const raw *xr = logits_row<DT>(P.logits, row);
-    const int64_t *ti = P.t_indices + int64_t(row) * K;
     for (int k = t; k < K; k += T) {
-      const int64_t id = ti[k];
+      const bool first = k == t;
+      const int64_t id = first ? id_first : P.t_indices[int64_t(row) * K + k];
       const bool in = id >= 0 && id < V;  // anything else is padding
-      float tv = load_any(P.t_values, int64_t(row) * K + k, int(P.t_dtype));
+      float tv = first ? tv_first : load_any(P.t_values, int64_t(row) * K + k, int(P.t_dtype));
       float xv = R::E::get(xr[in ? id : 0]);
       if (!in) tv = xv = kNegInf;
       t_idx[k] = in ? int(id) : -1;
@@ -263,7 +278,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
   if constexpr (TEACHER) {
     z_t += exp2_fast(float(rest2 - top2));
     if (z_t != 0.f) {
-      teach2 = log2(double(z_t));
+      teach2 = log2_fine(z_t);
       mass = 1.f;
       r = rest2 == -__builtin_inf() ? 0.f : exp2_fast(float(rest2 - top2 - teach2));
     }

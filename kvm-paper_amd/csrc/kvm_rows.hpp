@@ -87,6 +87,21 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
 }
 
+// Minimum / maximum of unsigned numbers over a wave, in every lane.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int l) { return uint32_t(__builtin_amdgcn_readlane(int(v), l)); }
+__device__ __forceinline__ uint32_t wave_min_u(uint32_t v) {
+  v = min(v, dpp_u<kDppRowRor8>(v));
+  v = min(v, dpp_u<kDppRowRor4>(v));
+  v = min(v, dpp_u<kDppQuadXor2>(v));
+  v = min(v, dpp_u<kDppQuadXor1>(v));
+  return min(min(lane_of(v, 0), lane_of(v, 16)), min(lane_of(v, 32), lane_of(v, 48)));
+}
+__device__ __forceinline__ uint32_t wave_max_u(uint32_t v) { return ~wave_min_u(~v); }
+
 // The same over the W <= 16 partial results of a workgroup's waves, part[0],
 // part[stride], ...: one LDS read per lane, the same value in every lane.
 template <int W>
@@ -176,6 +191,35 @@ struct Row {
         }
       }
       if (edge_idx >= 0 && (f(edge_idx, 1) & 1)) edge = kNegInf;
+    }
+  }
+
+  // each() of a row in registers, whose values that f returns as bits become
+  // -infinity for the passes after it.
+  template <class F>
+  __device__ __forceinline__ void take(F &&f) {
+    static_assert(NV > 0, "values of a row that is read again cannot be taken");
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (j * T < nfull) {
+        float x[N];
+        E::unpack(v[j], x);
+        const int c = j * T + t;
+        const uint32_t bits = f(x, head + c * N, c < nfull ? N : 0);
+        if (bits) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[i] = bits >> i & 1 ? kNegInf : x[i];
+          v[j] = E::pack(x);
+        }
+      }
+    }
+    if (edges && t < kWave) {
+      float x[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = kNegInf;
+      x[0] = edge;
+      if (f(x, edge_idx, edge_idx >= 0 ? 1 : 0)) edge = kNegInf;
     }
   }
 

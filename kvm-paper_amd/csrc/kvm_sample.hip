@@ -46,6 +46,7 @@ typedef unsigned long long u64;
 
 constexpr int kBins = 2048;
 constexpr int kCand = 1024;        // tokens that are ranked by counting
+constexpr int kFirst = 128;        // tokens that sampling without a small top-k looks at first
 constexpr int kMaxTop = 512;       // K of the top logits
 constexpr double kUnit = 4398046511104.0;  // 2^42
 
@@ -62,52 +63,61 @@ __device__ __forceinline__ u64 rank_of(uint32_t key, int idx) { return u64(key) 
 __device__ __forceinline__ int index_of(u64 rank) { return int(0xffffffffu - uint32_t(rank)); }
 __device__ __forceinline__ uint32_t key_part(u64 rank) { return uint32_t(rank >> 32); }
 
-// 2^(i / 64) for the weights' exponentials: the Taylor series of exp(f ln 2).
-constexpr int kTable = 64;
-__device__ __forceinline__ double exp2_fraction(int i) {
-#pragma clang fp contract(off)
-  const double f = double(i) * (0.6931471805599453 / kTable);
-  double p = 1.0, term = 1.0;
-  for (int k = 1; k <= 20; ++k) {
-    term *= f / double(k);
-    p += term;
+// 2^42 2^(i / 256), rounded from the Taylor series of exp(i ln 2 / 256).
+constexpr int kTable = 256;
+struct Powers {
+  double v[kTable];
+  constexpr Powers() : v() {
+    for (int i = 0; i < kTable; ++i) {
+      const double f = double(i) * (0.6931471805599453 / kTable);
+      double p = 1.0;
+      for (int k = 24; k >= 1; --k) p = 1.0 + p * f / double(k);
+      v[i] = p * kUnit;
+    }
   }
-  return p;
-}
+};
+__constant__ const Powers kPowers = Powers();
 
 // Weights and bins of a row at one temperature.
 struct Weights {
   float best;          // x_0
-  double per;          // 64 log2(e) / T
+  double per;          // 256 log2(e) / T
   float bins_per;      // bins per unit of logit
-  const double *table; // 2^(i / 64)
-  // floor(2^42 exp((x - best) / T) + 1/2): 2^(n / 64) from the table and the
-  // exponent, the rest by the Taylor series to the fifth power (|f| <= ln 2 /
-  // 128: off by less than 2^-54).  No contraction: a token's weight is the
+  const double *table; // kPowers in LDS
+  // 2^52 + floor(2^42 exp((x - best) / T) + 1/2) for a finite best: y = 256
+  // log2 of the exponential is a whole number n and f, |f| <= 1/2; 2^(n/256) is
+  // an entry of the table with its exponent moved, 2^(f/256) the Taylor series
+  // to the fourth power (off by less than 2^-54), and adding 2^52 to the
+  // product rounds it to a whole number in the low bits.  Weights below half a
+  // unit, of -infinity and NaN are 0.  No contraction: a token's weight is the
   // same wherever it is computed.
-  __device__ __forceinline__ u64 operator()(float x) const {
+  __device__ __forceinline__ double raised(float x) const {
 #pragma clang fp contract(off)
+    constexpr double kLn = 0.6931471805599453 / kTable;
     double y = (double(x) - double(best)) * per;
-    if (x == best) y = 0.0;  // infinity less itself
-    const bool some = y >= -43.0 * kTable;
-    if (!some) y = 0.0;
-    const double n = rint(y), f = (y - n) * (0.6931471805599453 / kTable);
-    double p = 1.0 / 120.0;
-    p = __builtin_fma(p, f, 1.0 / 24.0);
-    p = __builtin_fma(p, f, 1.0 / 6.0);
-    p = __builtin_fma(p, f, 0.5);
+    y = fmax(y, -44.0 * kTable);
+    const double shifted = y + 6755399441055744.0;  // 3 * 2^51: n in the low bits
+    const double f = y - (shifted - 6755399441055744.0);
+    const int n = int(__builtin_bit_cast(u64, shifted));
+    double p = kLn * kLn * kLn * kLn / 24.0;
+    p = __builtin_fma(p, f, kLn * kLn * kLn / 6.0);
+    p = __builtin_fma(p, f, kLn * kLn / 2.0);
+    p = __builtin_fma(p, f, kLn);
     p = __builtin_fma(p, f, 1.0);
-    p = __builtin_fma(p, f, 1.0);
-    const int k = int(n);
-    const double unit = __builtin_bit_cast(double, u64(1023 + 42 + (k >> 6)) << 52);  // 2^42 times the whole part
-    // Below 2^43: adding 2^52 rounds to a whole number in the low bits.
-    const double w = __builtin_fma(table[k & (kTable - 1)] * p, unit, 4503599627370496.0);
-    return some ? __builtin_bit_cast(u64, w) & 0xfffffffffffffull : 0;
+    u64 e = __builtin_bit_cast(u64, table[n & (kTable - 1)]);
+    e += u64(uint32_t(n & ~(kTable - 1)) << 12) << 32;  // the whole part of n / 256 into the exponent
+    return __builtin_fma(__builtin_bit_cast(double, e), p, 4503599627370496.0);
   }
+  __device__ __forceinline__ u64 operator()(float x) const {
+    if (best == __builtin_inff()) return x == best ? u64(kUnit) : 0;  // infinities share
+    return __builtin_bit_cast(u64, raised(x)) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ float place(float x) const { return (x == best ? 0.f : best - x) * bins_per; }
   __device__ __forceinline__ int bin(float x) const {
-    const float d = x == best ? 0.f : best - x;
-    return int(fminf(fmaxf(d * bins_per, 0.f), float(kBins - 1)));  // NaN (0 times infinity): 0
+    return int(fminf(fmaxf(place(x), 0.f), float(kBins - 1)));  // NaN (0 times infinity): 0
   }
+  // Whether a token may have a weight: false only for weights of 0.
+  __device__ __forceinline__ bool some(float x) const { return place(x) < float(kBins); }
 };
 
 struct Shared {
@@ -183,27 +193,35 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64 *red, u64 *total) {
 
 // Collects the values of a row with keys >= bound (in no particular order)
 // and returns how many there are; the list holds the first kCand of them.
-template <int T, class R>
-__device__ __forceinline__ int collect_above(const R &x, uint32_t bound, Shared &sh) {
+// TAKE: they leave the registers.
+template <int T, bool TAKE, class R>
+__device__ __forceinline__ int collect_above(R &x, uint32_t bound, Shared &sh) {
   constexpr int N = R::N;
   if (threadIdx.x == 0) sh.count = 0;
   __syncthreads();
   const float least = value_of(bound);
-  x.each([&](const float (&v)[N], int i0, int n) {
+  auto chunk = [&](const float (&v)[N], int i0, int n) -> uint32_t {
     float m = v[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
-    if (!(m < least)) {  // a NaN row part comes here too and is compared by key
+    uint32_t bits = 0;
+    if (!(m < least)) {  // nothing but NaN comes here too and is compared by key
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const uint32_t k = key_of(v[i]);
         if (i < n && k >= bound) {
+          bits |= 1u << i;
           const int at = atomicAdd(&sh.count, 1);
           if (at < kCand) sh.cand[at] = rank_of(k, i0 + i);
         }
       }
     }
-  });
+    return bits;
+  };
+  if constexpr (TAKE)
+    x.take(chunk);
+  else
+    x.each(chunk);
   __syncthreads();
   return sh.count;
 }
@@ -230,12 +248,7 @@ __device__ __forceinline__ uint32_t bound_of(float thread_max, int k, Shared &sh
       sh.bin = -1;
     }
     __syncthreads();
-    uint32_t lo = in ? mine : 0xffffffffu, hi = in ? mine : 0;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      lo = min(lo, uint32_t(__shfl_xor(int(lo), o)));
-      hi = max(hi, uint32_t(__shfl_xor(int(hi), o)));
-    }
+    uint32_t lo = wave_min_u(in ? mine : 0xffffffffu), hi = wave_max_u(in ? mine : 0);
     if ((t & 63) == 0) {
       atomicMin(&sh.kmin, lo);
       atomicMax(&sh.kmax, hi);
@@ -273,9 +286,7 @@ __device__ __forceinline__ uint32_t bound_of(float thread_max, int k, Shared &sh
     if (bin < 0) return none;  // fewer than k numbers
     above = sh.above;
     // the smallest maximum of that bin
-    uint32_t least = cut == bin ? mine : 0xffffffffu;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) least = min(least, uint32_t(__shfl_xor(int(least), o)));
+    const uint32_t least = wave_min_u(cut == bin ? mine : 0xffffffffu);
     if (t == 0) sh.kmin = 0xffffffffu;  // read by all before the last barrier
     __syncthreads();
     if ((t & 63) == 0) atomicMin(&sh.kmin, least);
@@ -300,6 +311,7 @@ __device__ __forceinline__ void ranked(int cnt, const Shared &sh, F &&f) {
     const int i = i0 + t / lanes;
     const u64 me = sh.cand[min(i, cnt - 1)];
     int r = 0;
+#pragma unroll 4
     for (int j = part; j < cnt; j += lanes) r += sh.cand[j] > me;
     for (int o = lanes / 2; o >= 1; o >>= 1) r += __shfl_xor(r, o);
     if (part == 0 && i < cnt) f(i, me, r);
@@ -379,6 +391,7 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
         const int i = min(i0 + t / lanes, cnt - 1);
         const u64 me = sh.cand[i];
         u64 before = 0;
+#pragma unroll 4
         for (int j = part; j < cnt; j += lanes)
           if (sh.cand[j] > me) before += sh.cw[j];
         for (int o = lanes / 2; o >= 1; o >>= 1) before += __shfl_xor(before, o);
@@ -473,12 +486,10 @@ __device__ __forceinline__ u64 build(const R &x, const Weights &wt, Shared &sh, 
   x.each([&](const float (&v)[N], int i0, int n) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (i < n && in(v[i], i0 + i)) {
-        const u64 w = wt(v[i]);
-        if (w) {
-          atomicAdd(&sh.hist[wt.bin(v[i])], COUNT ? 1 : w);
-          if (strong && double(w) >= least) big += w;
-        }
+      if (i < n && wt.some(v[i]) && in(v[i], i0 + i)) {
+        const u64 w = COUNT ? 1 : wt(v[i]);
+        if (w) atomicAdd(&sh.hist[wt.bin(v[i])], w);
+        if (strong && double(w) >= least) big += w;
       }
     }
   });
@@ -514,7 +525,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
   min_p = min_p > 0.f ? min_p : 0.f;
   const int top_k = P.top_k ? P.top_k[row] : int(P.top_k_all);
   const float u = P.uniforms[row];
-  if (t < kTable) sh.table[t] = exp2_fraction(t);
+  if (t < kTable) sh.table[t] = kPowers.v[t];
 
   float mine = kNegInf;
   x.each([&](const float (&v)[N], int, int) {
@@ -543,9 +554,9 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
   }
   Weights wt;
   wt.best = best;
-  wt.per = kTable * 1.4426950408889634 / double(temp);
+  wt.per = kTable * (1.4426950408889634 / double(temp));
   // 43 octaves of weight fill the bins
-  wt.bins_per = float(double(kBins) / (43.0 * 0.6931471805599453 * double(temp)));
+  wt.bins_per = float(fmin(double(kBins) / (43.0 * 0.6931471805599453 * double(temp)), 3e38));
   wt.table = sh.table;
   const double least = double(min_p) * kUnit;
   auto write = [&](u64 rank, u64 c) {  // one thread: the token and ln(w / C)
@@ -557,51 +568,97 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
   // The first tokens of the order.
   const bool some = top_k > 0 && top_k < V;  // top-k drops tokens
   const bool few = some && top_k <= T / 2;
-  const uint32_t bound = bound_of<T>(mine, few ? top_k : T / 4, sh);
-  const int cnt = collect_above<T>(x, bound, sh);
+  const uint32_t bound = bound_of<T>(mine, few ? top_k : kFirst, sh);
+  const int cnt = collect_above<T, false>(x, bound, sh);
   const bool covers = few || cnt == V;  // no token past the list is kept
-  if (cnt <= min(kCand, T) && (covers || !some)) {
-    u64 *sorted = sh.hist;
-    ranked<T>(cnt, sh, [&](int, u64 me, int r) { sorted[r] = me; });
+  if (cnt <= kCand && (covers || !some)) {
+    u64 *sorted = sh.hist, *weight = sh.hist + kCand;
+    ranked<T>(cnt, sh, [&](int, u64 me, int r) {
+      sorted[r] = me;
+      weight[r] = wt(value_of(key_part(me)));
+    });
     u64 z = 0, strong = 0;
     if (!covers) {  // the weight of the whole row
-      x.each([&](const float (&v)[N], int, int) {
+      u64 calls = 0;
+      if (min_p > 0.f) {
+        x.each([&](const float (&v)[N], int, int) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const u64 w = wt(v[i]);
-          z += w;
-          if (min_p > 0.f && double(w) >= least) strong += w;
-        }
-      });
+          for (int i = 0; i < N; ++i) {
+            const u64 w = wt(v[i]);
+            z += w;
+            if (double(w) >= least) strong += w;
+          }
+        });
+        strong = block_add<T>(strong, sh.scan);
+      } else if (best == __builtin_inff()) {
+        x.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) z += v[i] == best ? u64(kUnit) : 0;
+        });
+      } else {
+        // The bits of 2^52 + w are added up as they are; the constant part of
+        // every term is taken off modulo 2^64.
+        x.each([&](const float (&v)[N], int, int) {
+          calls += N;
+#pragma unroll
+          for (int i = 0; i < N; ++i) z += __builtin_bit_cast(u64, wt.raised(v[i]));
+        });
+        z -= calls * (u64(0x433) << 52);
+      }
       z = block_add<T>(z, sh.scan);
-      if (min_p > 0.f) strong = block_add<T>(strong, sh.scan);
     }
     __syncthreads();
-    const int k = some ? min(top_k, cnt) : cnt;
-    const u64 me = t < k ? sorted[t] : 0;  // one token per thread
-    const u64 w = t < k ? wt(value_of(key_part(me))) : 0;
-    u64 sum;
-    const u64 before = block_scan<T>(w, sh.scan, &sum);
-    if (covers) z = sum;
-    const double end = double(top_p) * double(z);
-    // The weight that is kept: inside the list as a sum of it, past it as one of the row.
-    const bool keep = t == 0 || (double(before) < end && double(w) >= least);
-    const u64 c_list = block_add<T>(keep ? w : 0, sh.scan);
-    u64 c = c_list;
-    bool known = true;
-    if (!covers) {
-      const bool p_in = top_p < 1.f && double(sum) >= end;
-      const bool m_in = min_p > 0.f && strong < sum;
-      if (!p_in && !m_in) {
-        known = top_p >= 1.f;
-        c = min_p > 0.f ? strong : z;
+    bool done = true;
+    if (t < kWave) {  // one wave finishes: consecutive tokens per lane, a prefix sum of their weights
+      const int k = some ? min(top_k, cnt) : cnt, per = (k + kWave - 1) / kWave;
+      const int first = min(t * per, k), last = min(first + per, k);
+      u64 own = 0;
+      for (int i = first; i < last; ++i) own += weight[i];
+      u64 before = own;
+#pragma unroll
+      for (int o = 1; o < kWave; o <<= 1) {
+        const u64 up = __shfl_up(before, o);
+        if (t >= o) before += up;
       }
+      const u64 sum = __shfl(before, kWave - 1);
+      before -= own;
+      if (covers) z = sum;
+      const double end = double(top_p) * double(z);
+      // What is kept of the list: each lane's last kept running sum, the largest of them.
+      u64 c = 0, run = before;
+      for (int i = first; i < last; ++i) {
+        const u64 w = weight[i];
+        if (i == 0 || (double(run) < end && double(w) >= least)) c = run + w;
+        run += w;
+      }
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) {
+        const u64 other = __shfl_xor(c, o);
+        c = other > c ? other : c;
+      }
+      if (!covers) {
+        // Past the list: the weight of the row, unless top-p or min-p ends inside it.
+        const bool p_in = top_p < 1.f && double(sum) >= end;
+        const bool m_in = min_p > 0.f && strong < sum;
+        if (!p_in && !m_in) {
+          done = top_p >= 1.f;
+          c = min_p > 0.f ? strong : z;
+        }
+      }
+      const u64 at = target_of(u, c);
+      done = done && at < sum;
+      if (done) {
+        run = before;
+        for (int i = first; i < last; ++i) {
+          const u64 w = weight[i];
+          if (at >= run && at < run + w) write(sorted[i], c);
+          run += w;
+        }
+      }
+      if (t == 0) sh.count = done;
     }
-    const u64 at = target_of(u, c);
-    if (known && at < sum) {
-      if (at >= before && at < before + w) write(me, c);
-      return;
-    }
+    __syncthreads();
+    if (sh.count) return;
   }
   auto all = [](float, int) { return true; };
   u64 limit = 0;  // the last token that top-k keeps (0: it keeps all)
@@ -609,15 +666,14 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
   if (some) {
     const u64 pre = build<T, true>(x, wt, sh, &z, 0.0, nullptr, all);
     if (u64(top_k) < z) {
-      auto positive = [&](float v, int) { return wt(v) != 0; };
-      locate<T, true>(x, wt, u64(top_k) - 1, pre, sh, positive);
+      locate<T, true>(x, wt, u64(top_k) - 1, pre, sh, [&](float v, int) { return wt.some(v); });
       limit = sh.found;
     }
   }
   auto kept = [&](float v, int i) { return limit == 0 || rank_of(key_of(v), i) >= limit; };
   u64 strong = 0;
   const u64 pre = build<T, false>(x, wt, sh, &z, least, min_p > 0.f ? &strong : nullptr, kept);
-  auto weighted = [&](float v, int i) { return kept(v, i) && wt(v) != 0; };
+  auto weighted = [&](float v, int i) { return wt.some(v) && kept(v, i) && wt(v) != 0; };
   u64 c = z;
 #pragma unroll 1
   for (int step = top_p < 1.f ? 0 : 1; step < 2; ++step) {  // where top-p ends, then the draw
@@ -655,9 +711,12 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
   });
   if (t == 0) s_next = 0;
   const uint32_t bound = bound_of<T>(mine, K, sh);
-  int cnt = collect_above<T>(x, bound, sh);
+  int cnt = collect_above<T, (NV > 0)>(x, bound, sh);
+  const bool many = cnt > kCand;
+  Row<DT, T, 0> again;  // for rows that are not in registers, or no longer whole there
+  if (NV == 0 || many) again.open(logits_row<DT>(L, row), V);
   u64 more_ties = 0;  // tokens of the K-th value behind it that are not in the list
-  if (cnt > kCand) {
+  if (many) {
     // Many equal or clustered logits: the K-th token by rank, then exactly K are collected.
     Weights wt;  // one bin: the tokens are cut by their keys from the start
     wt.best = 0.f;
@@ -666,10 +725,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
     wt.table = sh.table;
     __syncthreads();
     for (int i = t; i < kBins; i += T) sh.hist[i] = i ? 0 : u64(V);
-    auto all = [](float, int) { return true; };
-    Row<DT, T, 0> again;
-    again.open(logits_row<DT>(L, row), V);
-    locate<T, true>(again, wt, u64(K) - 1, t ? u64(V) : 0, sh, all);
+    locate<T, true>(again, wt, u64(K) - 1, t ? u64(V) : 0, sh, [](float, int) { return true; });
     const u64 last = sh.found;
     __syncthreads();
     if (t == 0) sh.count = 0;
@@ -694,8 +750,8 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
     more_ties = block_add<T>(ties, sh.scan);
     cnt = K;
   }
-  u64 in_list = 0;
-  ranked<T>(cnt, sh, [&](int, u64 me, int r) {
+  ranked<T>(cnt, sh, [&](int i, u64 me, int r) {
+    sh.cw[i] = u64(r);
     if (r < K) {
       static_cast<typename E::raw *>(values)[int64_t(row) * K + r] = E::put(value_of(key_part(me)));
       indices[int64_t(row) * K + r] = index_of(me);
@@ -706,36 +762,69 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
   if (!rest) return;
   __syncthreads();
   const u64 last = s_last, next = s_next;
-  const uint32_t kth = key_part(last);
-  for (int i = t; i < cnt; i += T) in_list += sh.cand[i] < last && key_part(sh.cand[i]) == kth;
-  const float ties = float(block_add<T>(in_list, sh.scan) + more_ties);
-  const float vk = value_of(kth);
   // The largest of the others: behind the K-th in the list, or below the list's bound.
-  float m = kNegInf;
-  if (next) {
-    m = value_of(key_part(next));
-  } else if (K < V) {
-    x.each([&](const float (&v)[N], int, int) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) m = fmaxf(m, v[i] < vk ? v[i] : kNegInf);
-    });
-    m = block_max<T>(m, sh.red);
-    if (ties > 0.f) m = vk;
-  }
-  const float ref = m == kNegInf ? 0.f : m;
+  float m = next ? value_of(key_part(next)) : kNegInf;
   float z = 0.f;
-  x.each([&](const float (&v)[N], int, int) {
+  double ref2;  // the sum's reference, in log2 units
+  if (NV > 0 && !many) {
+    if (!next) {
+      x.each([&](const float (&v)[N], int, int) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      z += __builtin_amdgcn_exp2f(v[i] < vk ? (v[i] - ref) * scale : kNegInf);
-  });
+        for (int i = 0; i < N; ++i) m = fmaxf(m, v[i]);
+      });
+      m = block_max<T>(m, sh.red);
+    }
+    const float ref = m == kNegInf ? 0.f : m, scaled = ref * scale;
+    if (fabsf(scaled) < 1e30f) {
+      ref2 = double(scaled);
+      auto term = [&](float v) { return __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -scaled)); };
+      x.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z += term(fmaxf(v[i], kNegInf));
+      });
+      for (int i = t; i < cnt; i += T)
+        if (sh.cw[i] >= u64(K)) z += term(value_of(key_part(sh.cand[i])));
+    } else {  // logits near the type's lowest value: subtracted before they are scaled
+      ref2 = double(ref) * scale;
+      auto term = [&](float v) { return __builtin_amdgcn_exp2f((v - ref) * scale); };
+      x.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z += term(fmaxf(v[i], kNegInf));
+      });
+      for (int i = t; i < cnt; i += T)
+        if (sh.cw[i] >= u64(K)) z += term(value_of(key_part(sh.cand[i])));
+    }
+  } else {
+    const uint32_t kth = key_part(last);
+    const float vk = value_of(kth);
+    u64 in_list = 0;
+    for (int i = t; i < cnt; i += T) in_list += sh.cand[i] < last && key_part(sh.cand[i]) == kth;
+    const float ties = float(block_add<T>(in_list, sh.scan) + more_ties);
+    if (!next && K < V) {
+      again.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = fmaxf(m, v[i] < vk ? v[i] : kNegInf);
+      });
+      m = block_max<T>(m, sh.red);
+      if (ties > 0.f) m = vk;
+    }
+    const float ref = m == kNegInf ? 0.f : m;
+    ref2 = double(ref) * scale;
+    again.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) z += __builtin_amdgcn_exp2f(v[i] < vk ? (v[i] - ref) * scale : kNegInf);
+    });
+    if (t == 0) z += ties;  // each of them is the reference itself: m = vk, exp = 1
+  }
   z = wave_add(z);
   __syncthreads();
   if ((t & 63) == 0) sh.red[t >> 6] = z;
   __syncthreads();
   if (t < 16) {
-    z = ties + part_add<T / kWave>(sh.red);  // each of the ties is the reference itself: m = vk, exp = 1
-    const double lse = m == kNegInf ? -__builtin_inf() : (double(ref) * scale + log2(double(z))) * 0.6931471805599453;
+    z = part_add<T / kWave>(sh.red);
+    const double lse = m == kNegInf ? -__builtin_inf()
+                       : m == __builtin_inff() ? __builtin_inf()
+                                               : (ref2 + log2(double(z))) * 0.6931471805599453;
     if (t == 0) rest[row] = float(lse);
   }
 }
