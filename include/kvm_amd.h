@@ -453,9 +453,9 @@ int kvm_sample(const kvm_sample_desc *d, void *stream);
  * outside [0, vocab) makes its row's loss and gradient NaN.
  * grad (optional, the logits' type, strides g_outer / g_inner, starting at the
  * same byte offset modulo 16 as the logits' row, for every row) receives
- * d loss / d x, times *inv_count where inv_count is given.  inv_count
- * (optional, written first): 1 / max(1, rows that count).  loss (optional):
- * the sum of row_loss, times *inv_count where that is given. */
+ * d loss / d x.  loss (optional): the sum of row_loss.  inv_count (optional):
+ * loss and grad are those of the mean, divided by max(1, rows that count);
+ * where there are labels, the word receives the reciprocal of that count. */
 typedef struct kvm_head_loss_desc {
   kvm_logits logits;
   const int64_t *labels;    /* [rows] or NULL (needs a teacher) */
@@ -468,7 +468,7 @@ typedef struct kvm_head_loss_desc {
   const float *t_rest;      /* [rows] or NULL */
   double temperature;
   float *row_loss;          /* out [rows] */
-  float *inv_count;         /* out [1] or NULL */
+  float *inv_count;         /* scratch [1], or NULL: no mean */
   float *loss;              /* out [1] or NULL */
   void *grad;               /* out or NULL */
   int64_t g_outer, g_inner;

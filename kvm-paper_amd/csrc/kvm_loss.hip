@@ -67,7 +67,7 @@ __device__ __forceinline__ double log2_of(double ref, float s) { return ref + lo
 __device__ __forceinline__ float reference(float m) { return m == kNegInf ? 0.f : m; }
 
 template <int DT, int T, int NV, bool TEACHER>
-__global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_head_loss(kvm_head_loss_desc P) {
+__global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_head_loss(kvm_head_loss_desc P, float every_row) {
   using R = Row<DT, T, NV>;
   using raw = typename R::raw;
   constexpr int N = R::N, W = T / kWave;
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int row = blockIdx.x;
   const int V = int(P.logits.vocab), K = int(P.k);
-  float *const row_loss = static_cast<float *>(P.row_loss);
+  float *const row_loss = P.row_loss;
   raw *grad = nullptr;
   if (P.grad) {
     const int o = row / int(P.logits.inner), i = row - o * int(P.logits.inner);
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
     return;
   }
   const float a = P.labels ? float(P.label_weight) : 0.f;  // weight of the hard labels
-  float scale = P.inv_count ? *P.inv_count : 1.f;
+  float scale = P.inv_count && P.labels ? *P.inv_count : every_row;
   // A label outside the vocabulary (and not ignored) makes the row's loss and gradient NaN.
   const bool bad = P.labels && (label < 0 || label >= V);
   if (bad) {
@@ -360,12 +360,24 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
   }
 }
 
+// f(i) for i < n, 8 of a thread's indices at a time, so that their loads are
+// in flight together (one workgroup of 1024 threads).
+template <class F>
+__device__ __forceinline__ void strided(int64_t n, F &&f) {
+  int64_t i = threadIdx.x;
+  for (; i + 7 * 1024 < n; i += 8 * 1024) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f(i + k * 1024);
+  }
+  for (; i < n; i += 1024) f(i);
+}
+
 // One workgroup: counts the labels that are not ignored and writes
-// 1 / max(count, 1) (1 / rows without labels).
+// 1 / max(count, 1).
 __global__ __launch_bounds__(1024) void k_count_labels(const int64_t *labels, int64_t n, int64_t ignore, float *inv) {
   __shared__ int part[16];
   int s = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += labels[i] != ignore;
+  strided(n, [&](int64_t i) { s += labels[i] != ignore; });
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
@@ -379,10 +391,11 @@ __global__ __launch_bounds__(1024) void k_count_labels(const int64_t *labels, in
 
 // One workgroup: out = factor * sum of n row losses (fp64 sums in a fixed
 // order, rounded once).
-__global__ __launch_bounds__(1024) void k_sum_losses(const float *loss, int64_t n, const float *factor, float *out) {
+__global__ __launch_bounds__(1024) void k_sum_losses(const float *loss, int64_t n, const float *factor,
+                                                     float every_row, float *out) {
   __shared__ double part[16];
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += loss[i];
+  strided(n, [&](int64_t i) { s += loss[i]; });
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
@@ -390,7 +403,7 @@ __global__ __launch_bounds__(1024) void k_sum_losses(const float *loss, int64_t 
   if (threadIdx.x == 0) {
     double c = 0.0;
     for (int w = 0; w < 16; ++w) c += part[w];
-    *out = float(c * (factor ? double(*factor) : 1.0));
+    *out = float(c * double(factor ? *factor : every_row));
   }
 }
 
@@ -427,6 +440,7 @@ __global__ __launch_bounds__(256) void k_scale_rows(void *data, int64_t rows, in
 
 struct LossLaunch {
   const kvm_head_loss_desc &P;
+  float every_row;
   hipStream_t stream;
   hipError_t err = hipSuccess;
 
@@ -434,7 +448,7 @@ struct LossLaunch {
   void run() {
     const dim3 grid(unsigned(P.logits.outer * P.logits.inner));
     if (P.k == 0) {
-      hipLaunchKernelGGL((k_head_loss<DT, T, NV, false>), grid, dim3(T), 0, stream, P);
+      hipLaunchKernelGGL((k_head_loss<DT, T, NV, false>), grid, dim3(T), 0, stream, P, every_row);
     } else {
       const size_t words = size_t(P.logits.vocab + 2 * Elem<DT>::N + 31) / 32;
       const size_t lds = (words + 3) / 4 * 16 + size_t(P.k) * 12;
@@ -443,7 +457,7 @@ struct LossLaunch {
                                   hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
         if (err != hipSuccess) return;
       }
-      hipLaunchKernelGGL((k_head_loss<DT, T, NV, true>), grid, dim3(T), lds, stream, P);
+      hipLaunchKernelGGL((k_head_loss<DT, T, NV, true>), grid, dim3(T), lds, stream, P, every_row);
     }
     err = hipGetLastError();
   }
@@ -455,20 +469,16 @@ int64_t head_loss_max_teacher() { return kMaxTeacher; }
 
 hipError_t launch_head_loss(const kvm_head_loss_desc &P, hipStream_t stream) {
   const int64_t rows = P.logits.outer * P.logits.inner;
-  if (P.inv_count && P.labels)
+  // A mean's factor: counted from the labels, or known.
+  const float *counted = P.labels ? P.inv_count : nullptr;
+  const float every_row = P.inv_count && !P.labels ? 1.f / float(rows) : 1.f;
+  if (counted)
     hipLaunchKernelGGL(k_count_labels, dim3(1), dim3(1024), 0, stream, P.labels, rows, P.ignore_index, P.inv_count);
-  else if (P.inv_count) {
-    const float inv = 1.f / float(rows);
-    const hipError_t e = launch_fill_u32(reinterpret_cast<unsigned *>(P.inv_count), 1,
-                                         __builtin_bit_cast(unsigned, inv), stream);
-    if (e != hipSuccess) return e;
-  }
-  LossLaunch l{P, stream};
+  LossLaunch l{P, every_row, stream};
   with_row(P.logits.vocab, P.logits.dtype, 256, l);
   if (l.err != hipSuccess) return l.err;
   if (P.loss)
-    hipLaunchKernelGGL(k_sum_losses, dim3(1), dim3(1024), 0, stream, static_cast<const float *>(P.row_loss), rows,
-                       static_cast<const float *>(P.inv_count), static_cast<float *>(P.loss));
+    hipLaunchKernelGGL(k_sum_losses, dim3(1), dim3(1024), 0, stream, P.row_loss, rows, counted, every_row, P.loss);
   return hipGetLastError();
 }
 

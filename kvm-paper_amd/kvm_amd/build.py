@@ -26,7 +26,7 @@ FLAGS = [
 ]
 
 
-OPS_SOURCE = "kvm_torch_ops.cpp"
+OPS_SOURCES = ["kvm_torch_ops.cpp", "kvm_logits_ops.cpp"]
 OPS_OUT = PKG / "libkvm_amd_torch.so"
 
 
@@ -43,7 +43,7 @@ def _run(cmd, verbose):
 
 
 def build_ops(verbose: bool = False) -> Path:
-    """The torch operator library (kvm_amd::prefill, kvm_amd::decode_step)
+    """The torch operator library (prefill, decode step, operators on logits)
     over libkvm_amd.so: host code only, against the installed ROCm torch."""
     import torch
     from torch.utils.cpp_extension import include_paths
@@ -52,7 +52,7 @@ def build_ops(verbose: bool = False) -> Path:
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     tmp = OPS_OUT.with_suffix(".so.tmp")
     cmd = [HIPCC, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           *[f"-I{p}" for p in include_paths(device_type="cuda")], "-o", str(tmp), str(CSRC / OPS_SOURCE),
+           *[f"-I{p}" for p in include_paths(device_type="cuda")], "-o", str(tmp), *[str(CSRC / s) for s in OPS_SOURCES],
            f"-L{PKG}", "-lkvm_amd", f"-L{torch_lib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch",
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
     _run(cmd, verbose)
