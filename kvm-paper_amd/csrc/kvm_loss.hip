@@ -45,6 +45,17 @@ __device__ __forceinline__ float load_any(const void *p, int64_t i, int dtype) {
   return dtype == KVM_BF16 ? Elem<KVM_BF16>::get(b) : Elem<KVM_F16>::get(b);
 }
 
+// A value that is the same in every lane, held once per wave.
+__device__ __forceinline__ float uniform(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+__device__ __forceinline__ double uniform(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint64_t lo = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(b))));
+  const uint64_t hi = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(b >> 32))));
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // log2(z) of a sum z >= 1 or so, off by about 2e-7 whatever its size: the
@@ -206,27 +217,40 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
   // row's maximum m (the teacher's to its own, top2): logits are subtracted
   // before they are scaled and before they meet a logarithm, so that rows of
   // the type's lowest value neither overflow nor swallow it.
-  const double m = reference(fmaxf(m_o, m_x));
-  m_o = reference(m_o);
-  m_x = reference(m_x);
+  const double m = uniform(reference(fmaxf(m_o, m_x)));
+  m_o = uniform(reference(m_o));
+  m_x = uniform(reference(m_x));
   const double rest2 = TEACHER && P.t_rest ? double(P.t_rest[row]) * 1.4426950408889634 : -__builtin_inf();
   double top2 = fmax(double(m_t) * c, rest2);
   if (top2 == -__builtin_inf()) top2 = 0.0;
-  // exp(v - m_o) from e = exp((v - m_o) / T): a power of it for the usual whole T.
-  const int whole = tau == 2.f ? 2 : tau == 4.f ? 4 : 0;
-  auto at_one = [&](float v, float e) -> float {
-    if (whole == 0) return exp2_fast((v - m_o) * kLog2e);
+  // The exponentials at T and, where hard labels need a softmax of their own,
+  // at 1: one, or both, the second a power of the first for the usual whole T.
+  // Each way has its own code, chosen once.
+  enum Way { kOne, kBoth, kSquare, kFourth };
+  const Way way = !two ? kOne : tau == 2.f ? kSquare : tau == 4.f ? kFourth : kBoth;
+  auto chosen = [&](auto &&f) {
+    if constexpr (TEACHER) {
+      if (way == kBoth) return f(std::integral_constant<Way, kBoth>{});
+      if (way == kSquare) return f(std::integral_constant<Way, kSquare>{});
+      if (way == kFourth) return f(std::integral_constant<Way, kFourth>{});
+    }
+    return f(std::integral_constant<Way, kOne>{});
+  };
+  auto at_one = [&](auto w, float v, float e) -> float {  // exp(v - m_o) from e = exp((v - m_o) / T)
+    if constexpr (decltype(w)::value == kBoth) return exp2_fast((v - m_o) * kLog2e);
     const float e2 = e * e;
-    return whole == 2 ? e2 : e2 * e2;
+    return decltype(w)::value == kSquare ? e2 : e2 * e2;
   };
   float z_o = 0.f, z_o1 = 0.f, z_t = 0.f, z_x = 0.f, z_x1 = 0.f;
-  others([&](const float (&v)[N], int, int) {
+  chosen([&](auto w) {
+    others([&](const float (&v)[N], int, int) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float e = exp2_fast((v[i] - m_o) * c);
-      z_o += e;
-      if (two) z_o1 += at_one(v[i], e);
-    }
+      for (int i = 0; i < N; ++i) {
+        const float e = exp2_fast((v[i] - m_o) * c);
+        z_o += e;
+        if constexpr (decltype(w)::value != kOne) z_o1 += at_one(w, v[i], e);
+      }
+    });
   });
   // The lowest of the entries that name a token stands for it in the student's sums.
   auto first_of = [&](int k) -> bool {
@@ -269,18 +293,19 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
   }
   // ---- logarithms of the row's sums (log2 units, relative to m)
   const double off_o = double(m_o) - m, off_x = double(m_x) - m;
-  const double others2 = log2_of(off_o * c, z_o);  // log Z_o
-  const double lse2 = TEACHER ? log2_add(others2, log2_of(off_x * c, z_x)) : others2;
-  const double lse21 = two ? log2_add(log2_of(off_o * kLog2e, z_o1), log2_of(off_x * kLog2e, z_x1)) : lse2;
+  const double others2 = uniform(log2_of(off_o * c, z_o));  // log Z_o
+  const double lse2 = uniform(TEACHER ? log2_add(others2, log2_of(off_x * c, z_x)) : others2);
+  const double lse21 =
+      two ? uniform(log2_add(log2_of(off_o * kLog2e, z_o1), log2_of(off_x * kLog2e, z_x1))) : lse2;
   // The teacher: its sum; its probability of the tokens it does not name; 1, or 0 for an empty teacher.
   double teach2 = 0.0;
   float r = 0.f, mass = 0.f;
   if constexpr (TEACHER) {
     z_t += exp2_fast(float(rest2 - top2));
     if (z_t != 0.f) {
-      teach2 = log2_fine(z_t);
+      teach2 = uniform(log2_fine(z_t));
       mass = 1.f;
-      r = rest2 == -__builtin_inf() ? 0.f : exp2_fast(float(rest2 - top2 - teach2));
+      r = uniform(rest2 == -__builtin_inf() ? 0.f : exp2_fast(float(rest2 - top2 - teach2)));
     }
   }
   // ---- loss
@@ -321,20 +346,24 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
     f *= w_soft;
   }
   if (hard) (two ? f1 : f) += w_hard * exp2_fast(float(off_o * (two ? kLog2e : c) - lse21));
-  auto other = [&](float v) -> float {
+  f = uniform(f);
+  f1 = uniform(f1);
+  auto other = [&](auto w, float v) -> float {
     const float e = exp2_fast((v - m_o) * c);
     float g = f * e;
-    if (two) g += f1 * at_one(v, e);
+    if constexpr (decltype(w)::value != kOne) g += f1 * at_one(w, v, e);
     return g;
   };
-  x.each([&](const float (&v)[N], int i0, int n) {
-    float g[N];
+  chosen([&](auto w) {
+    x.each([&](const float (&v)[N], int i0, int n) {
+      float g[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) g[i] = other(v[i]);
-    if (n == N)
-      *reinterpret_cast<uint4 *>(grad + i0) = R::E::pack(g);
-    else if (n == 1)
-      grad[i0] = R::E::put(g[0]);
+      for (int i = 0; i < N; ++i) g[i] = other(w, v[i]);
+      if (n == N)
+        *reinterpret_cast<uint4 *>(grad + i0) = R::E::pack(g);
+      else if (n == 1)
+        grad[i0] = R::E::put(g[0]);
+    });
   });
   __syncthreads();  // the tokens below are written over what the pass wrote there
   if constexpr (TEACHER) {
@@ -356,7 +385,8 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
   if (t == 0 && hard && !bad) {
     const int pos = x.shifted(int(label));
     const bool in_teacher = TEACHER && (bits[pos >> 5] >> (pos & 31) & 1);
-    if (!in_teacher) grad[label] = R::E::put(other(R::E::get(logits_row<DT>(P.logits, row)[label])) - w_hard);
+    const float v = x.at(int(label));
+    if (!in_teacher) grad[label] = R::E::put(chosen([&](auto w) { return other(w, v); }) - w_hard);
   }
 }
 
@@ -475,7 +505,7 @@ hipError_t launch_head_loss(const kvm_head_loss_desc &P, hipStream_t stream) {
   if (counted)
     hipLaunchKernelGGL(k_count_labels, dim3(1), dim3(1024), 0, stream, P.labels, rows, P.ignore_index, P.inv_count);
   LossLaunch l{P, every_row, stream};
-  with_row(P.logits.vocab, P.logits.dtype, 256, l);
+  with_row<true>(P.logits.vocab, P.logits.dtype, 256, l);
   if (l.err != hipSuccess) return l.err;
   if (P.loss)
     hipLaunchKernelGGL(k_sum_losses, dim3(1), dim3(1024), 0, stream, P.row_loss, rows, counted, every_row, P.loss);

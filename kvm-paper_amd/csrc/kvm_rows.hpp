@@ -8,6 +8,8 @@
 // lane of the first wave, so that no load touches memory outside the row.
 #pragma once
 
+#include <type_traits>
+
 #include "kvm_device.hpp"
 #include "kvm_internal.hpp"
 
@@ -121,18 +123,27 @@ __device__ __forceinline__ float part_max(const float *part, int stride = 1) {
 
 // A row of V values in the registers of a workgroup of T threads, NV chunks
 // per thread (NV = 0: read again on every pass; for rows that do not fit).
-template <int DT, int T, int NV>
+template <int DT, int T, int NV, bool FRESH = false>
 struct Row {
   using E = Elem<DT>;
   using raw = typename E::raw;
   static constexpr int N = E::N;
-  static constexpr int kBatch = 4;  // chunks of a thread in flight together when the row is read again
 
   uint4 v[NV > 0 ? NV : 1];
+  const raw *first;  // of the row
   const uint4 *chunks;
   int head, nfull, edges;  // values before the first chunk, whole chunks, values outside them
   int edge_idx;            // this lane's value outside the chunks (-1: none)
   float edge;
+
+  // Chunk j as it is in the registers.  FRESH: the compiler may not know that it
+  // is the value of an earlier pass, where it would keep the floats unpacked
+  // there, at two registers for every one that holds the row, and spill.
+  __device__ __forceinline__ uint4 held(int j) const {
+    uint4 u = v[j];
+    if constexpr (FRESH) asm volatile("" : "+v"(u.x), "+v"(u.y), "+v"(u.z), "+v"(u.w));
+    return u;
+  }
 
   __device__ __forceinline__ uint4 fetch(int c) const {
     const uint4 u = chunks[min(c, nfull - 1)];
@@ -148,6 +159,7 @@ struct Row {
   __device__ __forceinline__ void open(const raw *row, int V) {
     const int t = threadIdx.x;
     const int mis = int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(raw));
+    first = row;
     head = mis ? min(N - mis, V) : 0;
     nfull = (V - head) / N;
     edges = V - nfull * N;
@@ -166,6 +178,9 @@ struct Row {
     edge = edge_idx >= 0 ? E::get(row[edge_idx]) : kNegInf;
   }
 
+  // Value idx of the row, from memory.
+  __device__ __forceinline__ float at(int idx) const { return E::get(first[idx]); }
+
   // Position of value idx in an array that is laid out as the chunks are:
   // the first value of every chunk lies at a multiple of N.
   __device__ __forceinline__ int shifted(int idx) const { return idx + (head ? N - head : 0); }
@@ -183,7 +198,7 @@ struct Row {
           const uint32_t bits = c < nfull ? f(head + c * N, N) : 0;
           if (bits & ((1u << N) - 1)) {
             float x[N];
-            E::unpack(v[j], x);
+            E::unpack(held(j), x);
 #pragma unroll
             for (int i = 0; i < N; ++i) x[i] = bits >> i & 1 ? kNegInf : x[i];
             v[j] = E::pack(x);
@@ -194,7 +209,7 @@ struct Row {
     }
   }
 
-  // each() of a row in registers, whose values that f returns as bits become
+  // each() of a row in registers; chunks for which f returns true become
   // -infinity for the passes after it.
   template <class F>
   __device__ __forceinline__ void take(F &&f) {
@@ -204,14 +219,9 @@ struct Row {
     for (int j = 0; j < NV; ++j) {
       if (j * T < nfull) {
         float x[N];
-        E::unpack(v[j], x);
+        E::unpack(held(j), x);
         const int c = j * T + t;
-        const uint32_t bits = f(x, head + c * N, c < nfull ? N : 0);
-        if (bits) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) x[i] = bits >> i & 1 ? kNegInf : x[i];
-          v[j] = E::pack(x);
-        }
+        if (f(x, head + c * N, c < nfull ? N : 0)) v[j] = empty();
       }
     }
     if (edges && t < kWave) {
@@ -225,8 +235,10 @@ struct Row {
 
   // f(x, first, n): n values x[0..n) with indices first, first + 1, ...  n is
   // N, or 1 (a value outside the chunks), or 0 (none); the values past n are
-  // -infinity.  Chunks that no lane of the workgroup has are skipped.
-  template <class F>
+  // -infinity.  Chunks that no lane of the workgroup has are skipped.  A row
+  // that is read again is read BATCH chunks per thread at a time, one batch
+  // ahead of f, whose code is there BATCH times.
+  template <int BATCH = 4, class F>
   __device__ __forceinline__ void each(F &&f) const {
     const int t = threadIdx.x;
     if constexpr (NV > 0) {
@@ -234,20 +246,29 @@ struct Row {
       for (int j = 0; j < NV; ++j) {
         if (j * T < nfull) {
           float x[N];
-          E::unpack(v[j], x);
+          E::unpack(held(j), x);
           const int c = j * T + t;
           f(x, head + c * N, c < nfull ? N : 0);
         }
       }
     } else {
-      for (int c0 = t; c0 - t < nfull; c0 += T * kBatch) {
-        uint4 u[kBatch];
+      uint4 next[BATCH];
+      if (nfull > 0) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) u[i] = fetch(c0 + i * T);
+        for (int i = 0; i < BATCH; ++i) next[i] = fetch(t + i * T);
+      }
+#pragma unroll 1
+      for (int b = 0; b < nfull; b += T * BATCH) {  // chunks of the batch: b, b + 1, ...
+        uint4 u[BATCH];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int c = c0 + i * T;
-          if (c - t < nfull) {
+        for (int i = 0; i < BATCH; ++i) {
+          u[i] = next[i];
+          next[i] = fetch(b + T * (BATCH + i) + t);
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          const int c = b + i * T + t;
+          if (b + i * T < nfull) {
             float x[N];
             E::unpack(c < nfull ? u[i] : empty(), x);
             f(x, head + c * N, c < nfull ? N : 0);
@@ -280,24 +301,32 @@ inline bool row_resident(int64_t vocab, int64_t dtype) {
   return vocab <= int64_t(1024) * kRowChunks * (dtype == KVM_F32 ? 4 : 8);
 }
 
-// Calls f.template operator()<DT, T, NV>() for the variant of a row.
-template <class F>
+// Calls f.run<DT, T, NV>() for a row's type and length; RESIDENT false: for a
+// row that is read again whatever its length.
+template <bool RESIDENT, class F>
 void with_row(int64_t vocab, int64_t dtype, int64_t at_least, F &&f) {
-  const int t = row_threads(vocab, dtype, at_least);
-  const bool res = row_resident(vocab, dtype);
-#define KVM_ROW_DT(D)                                       \
-  if (!res) f.template run<D, 1024, 0>();                   \
-  else if (t == 256) f.template run<D, 256, kRowChunks>();  \
-  else if (t == 512) f.template run<D, 512, kRowChunks>();  \
-  else f.template run<D, 1024, kRowChunks>();
-  if (dtype == KVM_BF16) {
-    KVM_ROW_DT(KVM_BF16)
-  } else if (dtype == KVM_F16) {
-    KVM_ROW_DT(KVM_F16)
-  } else {
-    KVM_ROW_DT(KVM_F32)
-  }
-#undef KVM_ROW_DT
+  auto typed = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if constexpr (RESIDENT) {
+      const int t = row_threads(vocab, dtype, at_least);
+      if (row_resident(vocab, dtype)) {
+        if (t == 256)
+          f.template run<DT, 256, kRowChunks>();
+        else if (t == 512)
+          f.template run<DT, 512, kRowChunks>();
+        else
+          f.template run<DT, 1024, kRowChunks>();
+        return;
+      }
+    }
+    f.template run<DT, 1024, 0>();
+  };
+  if (dtype == KVM_BF16)
+    typed(std::integral_constant<int, KVM_BF16>{});
+  else if (dtype == KVM_F16)
+    typed(std::integral_constant<int, KVM_F16>{});
+  else
+    typed(std::integral_constant<int, KVM_F32>{});
 }
 
 }  // namespace kvm

@@ -33,9 +33,11 @@
 // more than 1024 tokens is cut again by their bit patterns until it has fewer,
 // or holds one value only, whose tokens rank by index.
 //
-// One workgroup per row.  The top logits hold the row in registers; sampling
-// reads it again on every pass, from the caches, in loops that are not unrolled
-// (with the fp64 exponentials in them they would not fit the instruction cache).
+// One workgroup per row, which is read once, into registers; locating reads it
+// again, from the caches, in loops that are not unrolled (a pass over registers
+// has its code once per chunk).
+
+#include <type_traits>
 
 #include "kvm_rows.hpp"
 
@@ -191,48 +193,96 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64 *red, u64 *total) {
   return before + s - v;
 }
 
-// Collects the values of a row with keys >= bound (in no particular order)
-// and returns how many there are; the list holds the first kCand of them.
-// TAKE: they leave the registers.
+// The chunks of a row that hold a value >= least, as collect_above lists them:
+// packed in sh.hist, with the first token and the number of values in sh.cw.
+struct Hits {
+  int chunks;   // in the list
+  float least;
+  bool every;   // NaN and -infinity too
+  // f(value, token, whether it is one of those >= least) for the list's values.
+  template <int T, class E, class F>
+  __device__ __forceinline__ void each(const Shared &sh, F &&f) const {
+    for (int i = threadIdx.x; i < chunks * E::N; i += T) {
+      const uint32_t tag = reinterpret_cast<const uint32_t *>(sh.cw)[i / E::N];
+      const int e = i % E::N;
+      if (e < int(tag >> 24)) {
+        const float v = E::get(reinterpret_cast<const typename E::raw *>(sh.hist)[i]);
+        f(v, int(tag & 0xffffff) + e, v >= least || every);
+      }
+    }
+  }
+};
+constexpr int kHitChunks = 1024;
+
+// Collects the tokens of a row with keys >= bound (in no particular order) and
+// returns how many there are; the list holds the first kCand of them (more
+// than kCand where their chunks do not fit either).  A pass over a row has its
+// code once per chunk, so a chunk with such a token only goes to LDS; its
+// tokens are looked at from there.  TAKE: those chunks leave the registers.
 template <int T, bool TAKE, class R>
-__device__ __forceinline__ int collect_above(R &x, uint32_t bound, Shared &sh) {
+__device__ __forceinline__ int collect_above(R &x, uint32_t bound, Shared &sh, Hits *hits) {
   constexpr int N = R::N;
-  if (threadIdx.x == 0) sh.count = 0;
+  uint4 *const chunks = reinterpret_cast<uint4 *>(sh.hist);
+  uint32_t *const tags = reinterpret_cast<uint32_t *>(sh.cw);
+  if (threadIdx.x == 0) sh.count = sh.above = 0;
   __syncthreads();
   const float least = value_of(bound);
-  auto chunk = [&](const float (&v)[N], int i0, int n) -> uint32_t {
+  const bool every = least == kNegInf;
+  auto chunk = [&](const float (&v)[N], int i0, int n) -> bool {
     float m = v[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
-    uint32_t bits = 0;
-    if (!(m < least)) {  // nothing but NaN comes here too and is compared by key
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t k = key_of(v[i]);
-        if (i < n && k >= bound) {
-          bits |= 1u << i;
-          const int at = atomicAdd(&sh.count, 1);
-          if (at < kCand) sh.cand[at] = rank_of(k, i0 + i);
-        }
+    const bool hit = (m >= least || every) && n > 0;
+    if (hit) {
+      const int at = atomicAdd(&sh.above, 1);
+      if (at < kHitChunks) {
+        chunks[at] = R::E::pack(v);
+        tags[at] = uint32_t(n) << 24 | uint32_t(i0);
       }
     }
-    return bits;
+    return hit;
   };
   if constexpr (TAKE)
     x.take(chunk);
   else
     x.each(chunk);
   __syncthreads();
+  *hits = {min(sh.above, kHitChunks), least, every};
+  if (sh.above > kHitChunks) return kCand + 1;
+  hits->template each<T, typename R::E>(sh, [&](float v, int idx, bool of_them) {
+    if (of_them) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCand) sh.cand[at] = rank_of(key_of(v), idx);
+    }
+  });
+  __syncthreads();
   return sh.count;
 }
 
-// A lower bound of the k-th largest key of the row: one of the threads' maxima
-// that k of them or a few more reach, from a histogram of the maxima over 256
-// bins, twice.  Where fewer than k threads hold a number, -infinity's key.
+// Inclusive prefix sum over a wave: shifts within rows of 16 lanes, then the
+// rows' totals across (DPP row_shr, row_bcast).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
+  return v;
+}
+
+// A lower bound of the k-th largest key of the row that k of the threads'
+// maxima or a few more reach: the edge of a bin of a histogram of the maxima
+// over 256 bins, cut once more where that bin is too full.  Where fewer than k
+// threads hold a number, -infinity's key.
 template <int T>
 __device__ __forceinline__ uint32_t bound_of(float thread_max, int k, Shared &sh) {
-  constexpr int kCuts = 256;
-  uint32_t *hist = reinterpret_cast<uint32_t *>(sh.fine);
+  constexpr int kCuts = 256, PER = kCuts / kWave;
+  uint32_t *hist = reinterpret_cast<uint32_t *>(sh.fine), *least = hist + kCuts, *most = least + 16;
   const int t = threadIdx.x;
   const uint32_t mine = key_of(thread_max), none = 0x007fffffu;  // -infinity's
   bool in = mine != none;
@@ -240,41 +290,33 @@ __device__ __forceinline__ uint32_t bound_of(float thread_max, int k, Shared &sh
   uint32_t bound = none;
 #pragma unroll 1
   for (int level = 0; level < 2; ++level) {
-    __syncthreads();
+    if (level) __syncthreads();
     for (int i = t; i < kCuts; i += T) hist[i] = 0;
-    if (t == 0) {
-      sh.kmin = 0xffffffffu;
-      sh.kmax = 0;
-      sh.bin = -1;
-    }
-    __syncthreads();
     uint32_t lo = wave_min_u(in ? mine : 0xffffffffu), hi = wave_max_u(in ? mine : 0);
     if ((t & 63) == 0) {
-      atomicMin(&sh.kmin, lo);
-      atomicMax(&sh.kmax, hi);
+      least[t >> 6] = lo;
+      most[t >> 6] = hi;
     }
+    if (t == 0) sh.bin = -1;
     __syncthreads();
-    lo = sh.kmin;
-    hi = sh.kmax;
-    const float per = float(kCuts) / (float(hi - lo) + 1.f);
+    const int l = t & 15;
+    lo = l < T / kWave ? least[l] : 0xffffffffu;
+    hi = l < T / kWave ? most[l] : 0;
+    lo = wave_min_u(lo);
+    hi = wave_max_u(hi);
+    const float span = float(hi - lo) + 1.f, per = float(kCuts) / span;
     const int cut = in ? min(int(float(hi - mine) * per), kCuts - 1) : kCuts;
     if (in) atomicAdd(&hist[cut], 1u);
     __syncthreads();
     if (t < kWave) {
-      uint32_t q[kCuts / kWave], own = 0;
+      uint32_t q[PER], own = 0;
 #pragma unroll
-      for (int i = 0; i < kCuts / kWave; ++i) own += q[i] = hist[t * (kCuts / kWave) + i];
-      uint32_t s = own;
+      for (int i = 0; i < PER; ++i) own += q[i] = hist[t * PER + i];
+      uint32_t s = above + wave_scan(own) - own;
 #pragma unroll
-      for (int o = 1; o < kWave; o <<= 1) {
-        const uint32_t up = __shfl_up(s, o);
-        if (t >= o) s += up;
-      }
-      s += above - own;
-#pragma unroll
-      for (int i = 0; i < kCuts / kWave; ++i) {
+      for (int i = 0; i < PER; ++i) {
         if (int(s) < k && int(s + q[i]) >= k) {
-          sh.bin = t * (kCuts / kWave) + i;
+          sh.bin = t * PER + i;
           sh.above = int(s);
           sh.count = int(s + q[i]);
         }
@@ -285,13 +327,9 @@ __device__ __forceinline__ uint32_t bound_of(float thread_max, int k, Shared &sh
     const int bin = sh.bin, reach = sh.count;
     if (bin < 0) return none;  // fewer than k numbers
     above = sh.above;
-    // the smallest maximum of that bin
-    const uint32_t least = wave_min_u(cut == bin ? mine : 0xffffffffu);
-    if (t == 0) sh.kmin = 0xffffffffu;  // read by all before the last barrier
-    __syncthreads();
-    if ((t & 63) == 0) atomicMin(&sh.kmin, least);
-    __syncthreads();
-    bound = sh.kmin;
+    // The bin's lower edge: 2^-20 of the distance below where the fp32 cuts put it, to be on the safe side.
+    const float below = float(bin + 1) * (span / float(kCuts)) * 1.000001f + 2.f;
+    bound = below < float(hi - none) ? hi - uint32_t(below) : none;
     if (reach <= k + k / 4 + 8) break;
     in = cut == bin;
   }
@@ -318,60 +356,78 @@ __device__ __forceinline__ void ranked(int cnt, const Shared &sh, F &&f) {
   }
 }
 
+// What is located: a rank among all tokens (one bin), a rank among the tokens
+// that may have a weight, or a running sum of weights.
+enum Quantity { kEvery, kCounted, kWeighed };
+
+// The tokens of a chunk that lie in a bin, as bits.
+template <Quantity Q, int N>
+__device__ __forceinline__ uint32_t in_bin(const Weights &wt, const float (&v)[N], int n, int bin) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float p = wt.place(v[i]);
+    bits |= (Q == kEvery || (p >= float(bin) && p < float(bin + 1))) && i < n ? 1u << i : 0u;
+  }
+  return bits;
+}
+
 // The token at running sum `target` (before <= target < before + its own) in
-// the order of the row, of weights (COUNT: of ones).  hist: the quantity per
-// bin of the row, which has been built; mine: this thread's exclusive prefix of
-// it.  Writes sh.found and sh.found_end.  in(x) selects values with a positive
-// quantity; every thread gets here.
-template <int T, bool COUNT, class R, class In>
-__device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target, u64 mine, Shared &sh, In &&in) {
+// the order of the row.  hist: the quantity per bin, which has been built;
+// mine: this thread's exclusive prefix of it; limit (kWeighed; 0: none): the
+// last token that counts.  Writes sh.found and sh.found_end; every thread
+// gets here.
+template <int T, Quantity Q, class R>
+__device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target, u64 mine, u64 limit, Shared &sh) {
   constexpr int N = R::N, PER = kBins / T;
   const int t = threadIdx.x;
-  // the bin
-  __syncthreads();
-  {
-    u64 s = mine;
+  auto amount = [&](float v) -> u64 { return Q == kWeighed ? wt(v) : 1; };
+  // Names the bin of `list` that holds the target; s: the sum before this thread's bins.
+  auto choose = [&](const u64 *list, u64 s) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const u64 q = sh.hist[t * PER + i];
+      const u64 q = list[t * PER + i];
       if (target >= s && target < s + q) {
         sh.bin = t * PER + i;
         sh.base = s;
       }
       s += q;
     }
-  }
-  if (t == 0) {
-    sh.count = 0;
-    sh.kmin = 0xffffffffu;
-    sh.kmax = 0;
-  }
+    if (t == 0) {
+      sh.count = 0;
+      sh.kmin = 0xffffffffu;
+      sh.kmax = 0;
+    }
+    __syncthreads();
+  };
   __syncthreads();
+  choose(sh.hist, mine);
   const int bin = sh.bin;
   u64 base = sh.base;
-  uint32_t lo = 0, hi = 0xffffffffu;  // keys of the tokens in question
-  bool first = true;
-  uint32_t f_hi = 0, f_span = 0;
-  int f_bin = 0;
-  while (true) {
-    // collect the tokens of the (sub-)bin, with their smallest and largest key
-    uint32_t a = 0xffffffffu, b = 0;
-    x.each([&](const float (&v)[N], int i0, int n) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i < n) {
-          if (wt.bin(v[i]) != bin) continue;
-          const uint32_t k = key_of(v[i]);
-          bool hit = k >= lo && k <= hi;
-          if (hit && !first) hit = int(u64(f_hi - k) * kBins / (u64(f_span) + 1)) == f_bin;
-          if (hit && in(v[i], i0 + i)) {
-            a = min(a, k);
-            b = max(b, k);
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kCand) sh.cand[at] = rank_of(k, i0 + i);
-          }
-        }
+  // The tokens in question: those of the bin with keys in [lo, hi] and, past
+  // the first cut, in part f_part of kBins equal parts of [f_hi - f_span, f_hi].
+  uint32_t lo = 0, hi = 0xffffffffu, f_hi = 0, f_span = 0;
+  int f_part = -1;
+  auto part_of = [&](uint32_t k) { return int(u64(f_hi - k) * kBins / (u64(f_span) + 1)); };
+  auto tokens = [&](auto &&f) {  // f(key, index, value) for each of them
+    x.template each<1>([&](const float (&v)[N], int i0, int n) {
+      for (uint32_t bits = in_bin<Q, N>(wt, v, n, bin); bits; bits &= bits - 1) {
+        const int idx = i0 + __ffs(bits) - 1;
+        const float xv = x.at(idx);
+        const uint32_t k = key_of(xv);
+        if (k >= lo && k <= hi && (f_part < 0 || part_of(k) == f_part) && rank_of(k, idx) >= limit) f(k, idx, xv);
       }
+    });
+  };
+#pragma unroll 1
+  while (true) {
+    // collect them, with their smallest and largest key
+    uint32_t a = 0xffffffffu, b = 0;
+    tokens([&](uint32_t k, int idx, float) {
+      a = min(a, k);
+      b = max(b, k);
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCand) sh.cand[at] = rank_of(k, idx);
     });
     if (a <= b) {
       atomicMin(&sh.kmin, a);
@@ -382,7 +438,7 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
     lo = sh.kmin;
     hi = sh.kmax;
     if (cnt <= kCand) {
-      for (int i = t; i < cnt; i += T) sh.cw[i] = COUNT ? 1 : wt(value_of(key_part(sh.cand[i])));
+      for (int i = t; i < cnt; i += T) sh.cw[i] = amount(value_of(key_part(sh.cand[i])));
       __syncthreads();
       int lanes = 1;
       while (lanes < 16 && 2 * lanes * cnt <= T) lanes *= 2;
@@ -406,16 +462,17 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
     }
     if (lo == hi) {
       // One value: the n-th of its tokens by index, found by bisection over the index.
-      const u64 w = COUNT ? 1 : wt(value_of(lo));
+      const u64 w = max(amount(value_of(lo)), u64(1));
       const u64 nth = (target - base) / w;
-      int below = -1, upto = (1 << 20) - 1;  // at most nth tokens are <= below, more than nth are <= upto
+      const int last = limit && key_part(limit) == lo ? index_of(limit) : 0x7fffffff;
+      int below = -1, upto = int(kMaxVocab) - 1;  // at most nth tokens are <= below, more than nth are <= upto
+#pragma unroll 1
       while (upto - below > 1) {
         const int mid = below + (upto - below) / 2;
         u64 c = 0;
-        x.each([&](const float (&v)[N], int i0, int n) {
+        x.template each<1>([&](const float (&v)[N], int i0, int n) {
 #pragma unroll
-          for (int i = 0; i < N; ++i)
-            if (i < n && i0 + i <= mid && key_of(v[i]) == lo && in(v[i], i0 + i)) ++c;
+          for (int i = 0; i < N; ++i) c += i < n && i0 + i <= min(mid, last) && key_of(v[i]) == lo;
         });
         c = block_add<T>(c, sh.scan);
         if (c > nth)
@@ -430,71 +487,48 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
       __syncthreads();
       return;
     }
-    // cut [lo, hi] into kBins by key, the largest keys first
+    // cut [lo, hi] into kBins parts, the largest keys first
     __syncthreads();
     for (int i = t; i < kBins; i += T) sh.fine[i] = 0;
     f_hi = hi;
     f_span = hi - lo;
+    f_part = -1;
     __syncthreads();
-    x.each([&](const float (&v)[N], int i0, int n) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (i >= n || wt.bin(v[i]) != bin) continue;
-        const uint32_t k = key_of(v[i]);
-        if (k >= lo && k <= hi && in(v[i], i0 + i))
-          atomicAdd(&sh.fine[int(u64(f_hi - k) * kBins / (u64(f_span) + 1))], COUNT ? 1 : wt(v[i]));
-      }
-    });
+    tokens([&](uint32_t k, int, float v) { atomicAdd(&sh.fine[part_of(k)], amount(v)); });
     __syncthreads();
     u64 own = 0, all;
 #pragma unroll
     for (int i = 0; i < PER; ++i) own += sh.fine[t * PER + i];
-    u64 s = base + block_scan<T>(own, sh.scan, &all);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const u64 q = sh.fine[t * PER + i];
-      if (target >= s && target < s + q) {
-        sh.bin = t * PER + i;
-        sh.base = s;
-      }
-      s += q;
-    }
-    if (t == 0) {
-      sh.count = 0;
-      sh.kmin = 0xffffffffu;
-      sh.kmax = 0;
-    }
-    __syncthreads();
-    f_bin = sh.bin;
+    choose(sh.fine, base + block_scan<T>(own, sh.scan, &all));
+    f_part = sh.bin;
     base = sh.base;
-    first = false;
   }
 }
 
-// Histogram of a row's weights (COUNT: of ones) over the values that in()
-// selects; returns this thread's exclusive prefix, *total the sum.  strong
-// (optional): the sum of the weights >= least.
-template <int T, bool COUNT, class R, class In>
-__device__ __forceinline__ u64 build(const R &x, const Weights &wt, Shared &sh, u64 *total, double least, u64 *strong,
-                                     In &&in) {
+// Histogram of a row's weights (kCounted: of ones) over the tokens down to
+// limit (0: all); returns this thread's exclusive prefix, *total the sum.
+// strong (optional): the sum of the weights >= least.
+template <int T, Quantity Q, class R>
+__device__ __forceinline__ u64 build(const R &x, const Weights &wt, u64 limit, Shared &sh, u64 *total, double least,
+                                     u64 *strong) {
   constexpr int N = R::N, PER = kBins / T;
   const int t = threadIdx.x;
   __syncthreads();
   for (int i = t; i < kBins; i += T) sh.hist[i] = 0;
   __syncthreads();
   u64 big = 0;
-  x.each([&](const float (&v)[N], int i0, int n) {
+  x.template each<1>([&](const float (&v)[N], int i0, int n) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (i < n && wt.some(v[i]) && in(v[i], i0 + i)) {
-        const u64 w = COUNT ? 1 : wt(v[i]);
-        if (w) atomicAdd(&sh.hist[wt.bin(v[i])], w);
-        if (strong && double(w) >= least) big += w;
+      const u64 w = Q == kCounted ? 1 : wt(v[i]);
+      if (i < n && wt.some(v[i]) && w && (limit == 0 || rank_of(key_of(v[i]), i0 + i) >= limit)) {
+        atomicAdd(&sh.hist[wt.bin(v[i])], w);
+        if (Q == kWeighed && strong && double(w) >= least) big += w;
       }
     }
   });
   __syncthreads();
-  if (strong) *strong = block_add<T>(big, sh.scan);
+  if (Q == kWeighed && strong) *strong = block_add<T>(big, sh.scan);
   u64 own = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) own += sh.hist[t * PER + i];
@@ -509,9 +543,9 @@ __device__ __forceinline__ u64 target_of(float u, u64 c) {
   return at >= double(last) ? last : u64(at);
 }
 
-template <int DT, int T>
+template <int DT, int T, int NV>
 __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_sample(kvm_sample_desc P) {
-  using R = Row<DT, T, 0>;
+  using R = Row<DT, T, NV, true>;
   constexpr int N = R::N;
   __shared__ Shared sh;
   const int t = threadIdx.x, row = blockIdx.x;
@@ -537,13 +571,15 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
     P.tokens[row] = token;
     if (P.logprobs) P.logprobs[row] = logprob;
   };
+  Row<DT, T, 0> again;  // the passes after the first two read the row again
+  again.open(logits_row<DT>(P.logits, row), V);
   if (best == kNegInf) {  // nothing to draw from
     if (t == 0) answer(0, __builtin_nanf(""));
     return;
   }
   if (!(temp > 0.f) || top_k == 1) {  // the first token of the order
     int at = 0x7fffffff;
-    x.each([&](const float (&v)[N], int i0, int n) {
+    again.each([&](const float (&v)[N], int i0, int n) {
 #pragma unroll
       for (int i = N - 1; i >= 0; --i)
         if (i < n && v[i] == best) at = min(at, i0 + i);
@@ -569,8 +605,11 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
   const bool some = top_k > 0 && top_k < V;  // top-k drops tokens
   const bool few = some && top_k <= T / 2;
   const uint32_t bound = bound_of<T>(mine, few ? top_k : kFirst, sh);
-  const int cnt = collect_above<T, false>(x, bound, sh);
+  Hits hits;
+  const int cnt = collect_above<T, false>(x, bound, sh, &hits);
   const bool covers = few || cnt == V;  // no token past the list is kept
+  // Whether min-p drops all tokens past the list, whose keys are below the bound.
+  const bool m_in = min_p > 0.f && double(wt(value_of(bound))) < least;
   if (cnt <= kCand && (covers || !some)) {
     u64 *sorted = sh.hist, *weight = sh.hist + kCand;
     ranked<T>(cnt, sh, [&](int, u64 me, int r) {
@@ -578,32 +617,33 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
       weight[r] = wt(value_of(key_part(me)));
     });
     u64 z = 0, strong = 0;
-    if (!covers) {  // the weight of the whole row
-      u64 calls = 0;
-      if (min_p > 0.f) {
-        x.each([&](const float (&v)[N], int, int) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const u64 w = wt(v[i]);
-            z += w;
-            if (double(w) >= least) strong += w;
-          }
-        });
-        strong = block_add<T>(strong, sh.scan);
-      } else if (best == __builtin_inff()) {
-        x.each([&](const float (&v)[N], int, int) {
+    // The weight of the row, unless min-p alone says where the kept tokens end.
+    if (!covers && !(m_in && top_p >= 1.f)) {
+      if (best == __builtin_inff()) {
+        again.template each<1>([&](const float (&v)[N], int, int) {
 #pragma unroll
           for (int i = 0; i < N; ++i) z += v[i] == best ? u64(kUnit) : 0;
         });
       } else {
         // The bits of 2^52 + w are added up as they are; the constant part of
         // every term is taken off modulo 2^64.
-        x.each([&](const float (&v)[N], int, int) {
+        u64 calls = 0;
+        again.template each<1>([&](const float (&v)[N], int, int) {
           calls += N;
 #pragma unroll
           for (int i = 0; i < N; ++i) z += __builtin_bit_cast(u64, wt.raised(v[i]));
         });
         z -= calls * (u64(0x433) << 52);
+      }
+      if (min_p > 0.f && !m_in) {
+        again.template each<1>([&](const float (&v)[N], int, int) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const u64 w = wt(v[i]);
+            strong += double(w) >= least ? w : 0;
+          }
+        });
+        strong = block_add<T>(strong, sh.scan);
       }
       z = block_add<T>(z, sh.scan);
     }
@@ -628,7 +668,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
       u64 c = 0, run = before;
       for (int i = first; i < last; ++i) {
         const u64 w = weight[i];
-        if (i == 0 || (double(run) < end && double(w) >= least)) c = run + w;
+        if (i == 0 || ((top_p >= 1.f || double(run) < end) && double(w) >= least)) c = run + w;
         run += w;
       }
 #pragma unroll
@@ -639,7 +679,6 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
       if (!covers) {
         // Past the list: the weight of the row, unless top-p or min-p ends inside it.
         const bool p_in = top_p < 1.f && double(sum) >= end;
-        const bool m_in = min_p > 0.f && strong < sum;
         if (!p_in && !m_in) {
           done = top_p >= 1.f;
           c = min_p > 0.f ? strong : z;
@@ -660,20 +699,17 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
     __syncthreads();
     if (sh.count) return;
   }
-  auto all = [](float, int) { return true; };
   u64 limit = 0;  // the last token that top-k keeps (0: it keeps all)
   u64 z;
   if (some) {
-    const u64 pre = build<T, true>(x, wt, sh, &z, 0.0, nullptr, all);
+    const u64 pre = build<T, kCounted>(again, wt, 0, sh, &z, 0.0, nullptr);
     if (u64(top_k) < z) {
-      locate<T, true>(x, wt, u64(top_k) - 1, pre, sh, [&](float v, int) { return wt.some(v); });
+      locate<T, kCounted>(again, wt, u64(top_k) - 1, pre, 0, sh);
       limit = sh.found;
     }
   }
-  auto kept = [&](float v, int i) { return limit == 0 || rank_of(key_of(v), i) >= limit; };
   u64 strong = 0;
-  const u64 pre = build<T, false>(x, wt, sh, &z, least, min_p > 0.f ? &strong : nullptr, kept);
-  auto weighted = [&](float v, int i) { return wt.some(v) && kept(v, i) && wt(v) != 0; };
+  const u64 pre = build<T, kWeighed>(again, wt, limit, sh, &z, least, min_p > 0.f ? &strong : nullptr);
   u64 c = z;
 #pragma unroll 1
   for (int step = top_p < 1.f ? 0 : 1; step < 2; ++step) {  // where top-p ends, then the draw
@@ -686,7 +722,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
       if (c < u64(kUnit)) c = u64(kUnit);  // the first token is always kept
       target = target_of(u, c);
     }
-    locate<T, false>(x, wt, target, pre, sh, weighted);
+    locate<T, kWeighed>(again, wt, target, pre, limit, sh);
     if (step == 0) c = sh.found_end;
   }
   if (t == 0) write(sh.found, c);
@@ -695,7 +731,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
 template <int DT, int T, int NV>
 __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_top_logits(kvm_logits L, int K, float scale, void *values, int64_t *indices,
                                                   float *rest) {
-  using R = Row<DT, T, NV>;
+  using R = Row<DT, T, NV, true>;
   using E = Elem<DT>;
   constexpr int N = R::N;
   __shared__ Shared sh;
@@ -711,8 +747,12 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
   });
   if (t == 0) s_next = 0;
   const uint32_t bound = bound_of<T>(mine, K, sh);
-  int cnt = collect_above<T, (NV > 0)>(x, bound, sh);
+  Hits hits;
+  int cnt = collect_above<T, (NV > 0)>(x, bound, sh, &hits);
   const bool many = cnt > kCand;
+  // Which tokens of the list are past the K-th.
+  if (NV > 0 && !many)
+    for (int i = t; i < cnt; i += T) sh.fine[i] = 0;
   Row<DT, T, 0> again;  // for rows that are not in registers, or no longer whole there
   if (NV == 0 || many) again.open(logits_row<DT>(L, row), V);
   u64 more_ties = 0;  // tokens of the K-th value behind it that are not in the list
@@ -725,13 +765,13 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
     wt.table = sh.table;
     __syncthreads();
     for (int i = t; i < kBins; i += T) sh.hist[i] = i ? 0 : u64(V);
-    locate<T, true>(again, wt, u64(K) - 1, t ? u64(V) : 0, sh, [](float, int) { return true; });
+    locate<T, kEvery>(again, wt, u64(K) - 1, t ? u64(V) : 0, 0, sh);
     const u64 last = sh.found;
     __syncthreads();
     if (t == 0) sh.count = 0;
     __syncthreads();
     u64 ties = 0;
-    again.each([&](const float (&v)[N], int i0, int n) {
+    again.template each<1>([&](const float (&v)[N], int i0, int n) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         if (i < n) {
@@ -751,7 +791,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
     cnt = K;
   }
   ranked<T>(cnt, sh, [&](int i, u64 me, int r) {
-    sh.cw[i] = u64(r);
+    if (NV > 0 && !many && r >= K) sh.fine[i] = 1;
     if (r < K) {
       static_cast<typename E::raw *>(values)[int64_t(row) * K + r] = E::put(value_of(key_part(me)));
       indices[int64_t(row) * K + r] = index_of(me);
@@ -772,8 +812,25 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
 #pragma unroll
         for (int i = 0; i < N; ++i) m = fmaxf(m, v[i]);
       });
+      hits.template each<T, E>(sh, [&](float v, int, bool of_them) {
+        if (!of_them) m = fmaxf(m, v);
+      });
       m = block_max<T>(m, sh.red);
     }
+    // What left the registers but is not among the K: the rest of those chunks,
+    // and of the list.  Both lists are in the order in which waves got there, so
+    // these terms (at most 1) are added up as whole multiples of 2^-40.
+    auto beside = [&](auto &&term) {
+      u64 units = 0;
+      auto add = [&](float v) { units += u64(term(v) * 1099511627776.f); };
+      hits.template each<T, E>(sh, [&](float v, int, bool of_them) {
+        if (!of_them) add(fmaxf(v, kNegInf));
+      });
+      for (int i = t; i < cnt; i += T)
+        if (sh.fine[i]) add(value_of(key_part(sh.cand[i])));
+      units = block_add<T>(units, sh.scan);
+      if (t == 0) z += float(double(units) / 1099511627776.0);
+    };
     const float ref = m == kNegInf ? 0.f : m, scaled = ref * scale;
     if (fabsf(scaled) < 1e30f) {
       ref2 = double(scaled);
@@ -782,8 +839,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
 #pragma unroll
         for (int i = 0; i < N; ++i) z += term(fmaxf(v[i], kNegInf));
       });
-      for (int i = t; i < cnt; i += T)
-        if (sh.cw[i] >= u64(K)) z += term(value_of(key_part(sh.cand[i])));
+      beside(term);
     } else {  // logits near the type's lowest value: subtracted before they are scaled
       ref2 = double(ref) * scale;
       auto term = [&](float v) { return __builtin_amdgcn_exp2f((v - ref) * scale); };
@@ -791,8 +847,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
 #pragma unroll
         for (int i = 0; i < N; ++i) z += term(fmaxf(v[i], kNegInf));
       });
-      for (int i = t; i < cnt; i += T)
-        if (sh.cw[i] >= u64(K)) z += term(value_of(key_part(sh.cand[i])));
+      beside(term);
     }
   } else {
     const uint32_t kth = key_part(last);
@@ -829,6 +884,17 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
   }
 }
 
+struct SampleLaunch {
+  const kvm_sample_desc &P;
+  hipStream_t stream;
+  template <int DT, int T, int NV>
+  void run() {
+    if constexpr (T >= 512)
+      hipLaunchKernelGGL((k_sample<DT, T, NV>), dim3(unsigned(P.logits.outer * P.logits.inner)), dim3(T), 0, stream,
+                         P);
+  }
+};
+
 struct TopLaunch {
   const kvm_logits &L;
   int K;
@@ -849,23 +915,15 @@ struct TopLaunch {
 int64_t top_logits_max() { return kMaxTop; }
 
 hipError_t launch_sample(const kvm_sample_desc &P, hipStream_t stream) {
-  // Up to one row per compute unit: 1024 threads finish a row soonest; more
-  // rows: workgroups of 512, two of which share a compute unit.
+  // More rows than compute units: the rows stay in registers.  Fewer: a pass's
+  // unrolled code would be read from memory by a workgroup that runs it once
+  // (one row of 50304: 54 us, against 23 with the row read again and loops).
   const int64_t rows = P.logits.outer * P.logits.inner;
-  const dim3 grid{unsigned(rows)};
-#define KVM_SAMPLE(D)                                                                \
-  if (rows <= 256)                                                                   \
-    hipLaunchKernelGGL((k_sample<D, 1024>), grid, dim3(1024), 0, stream, P);         \
-  else                                                                               \
-    hipLaunchKernelGGL((k_sample<D, 512>), grid, dim3(512), 0, stream, P);
-  if (P.logits.dtype == KVM_BF16) {
-    KVM_SAMPLE(KVM_BF16)
-  } else if (P.logits.dtype == KVM_F16) {
-    KVM_SAMPLE(KVM_F16)
-  } else {
-    KVM_SAMPLE(KVM_F32)
-  }
-#undef KVM_SAMPLE
+  SampleLaunch l{P, stream};
+  if (rows <= 256)
+    with_row<false>(P.logits.vocab, P.logits.dtype, 1024, l);
+  else
+    with_row<true>(P.logits.vocab, P.logits.dtype, 512, l);
   return hipGetLastError();
 }
 
@@ -873,7 +931,7 @@ hipError_t launch_top_logits(const kvm_logits &L, int64_t k, double temperature,
                              float *rest, hipStream_t stream) {
   TopLaunch l{L, int(k), float(1.4426950408889634 / temperature), values, indices, rest, stream};
   // At least twice as many threads as values: the bound from the threads' maxima then passes 1.4 K logits or fewer.
-  with_row(L.vocab, L.dtype, 2 * k, l);
+  with_row<true>(L.vocab, L.dtype, 2 * k, l);
   return hipGetLastError();
 }
 
