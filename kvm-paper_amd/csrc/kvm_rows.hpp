@@ -128,6 +128,7 @@ struct Row {
   using E = Elem<DT>;
   using raw = typename E::raw;
   static constexpr int N = E::N;
+  static constexpr bool kResident = NV > 0;
 
   uint4 v[NV > 0 ? NV : 1];
   const raw *first;  // of the row
@@ -209,27 +210,46 @@ struct Row {
     }
   }
 
-  // each() of a row in registers; chunks for which f returns true become
-  // -infinity for the passes after it.
-  template <class F>
-  __device__ __forceinline__ void take(F &&f) {
-    static_assert(NV > 0, "values of a row that is read again cannot be taken");
-    const int t = threadIdx.x;
+  // The largest value of each of this thread's chunks, and of all it holds (a
+  // NaN is passed over).
+  __device__ __forceinline__ float maxima(float (&most)[NV > 0 ? NV : 1]) const {
+    float m = edge;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      most[j] = kNegInf;
       if (j * T < nfull) {
         float x[N];
         E::unpack(held(j), x);
-        const int c = j * T + t;
-        if (f(x, head + c * N, c < nfull ? N : 0)) v[j] = empty();
+#pragma unroll
+        for (int i = 0; i < N; ++i) most[j] = fmaxf(most[j], x[i]);
+        m = fmaxf(m, most[j]);
       }
     }
-    if (edges && t < kWave) {
+    return m;
+  }
+
+  // f(x, first, n) for the chunks (and values outside them) whose maxima are
+  // >= least, or for all of them.  TAKE: they become -infinity.
+  template <bool TAKE, class F>
+  __device__ __forceinline__ void above(const float (&most)[NV > 0 ? NV : 1], float least, bool all, F &&f) {
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = j * T + t;
+      if ((most[j] >= least || all) && c < nfull) {
+        float x[N];
+        E::unpack(held(j), x);
+        f(x, head + c * N, N);
+        if constexpr (TAKE) v[j] = empty();
+      }
+    }
+    if (edge_idx >= 0 && (edge >= least || all)) {
       float x[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) x[i] = kNegInf;
       x[0] = edge;
-      if (f(x, edge_idx, edge_idx >= 0 ? 1 : 0)) edge = kNegInf;
+      f(x, edge_idx, 1);
+      if constexpr (TAKE) edge = kNegInf;
     }
   }
 

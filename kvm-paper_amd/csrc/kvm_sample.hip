@@ -219,8 +219,8 @@ constexpr int kHitChunks = 1024;
 // than kCand where their chunks do not fit either).  A pass over a row has its
 // code once per chunk, so a chunk with such a token only goes to LDS; its
 // tokens are looked at from there.  TAKE: those chunks leave the registers.
-template <int T, bool TAKE, class R>
-__device__ __forceinline__ int collect_above(R &x, uint32_t bound, Shared &sh, Hits *hits) {
+template <int T, bool TAKE, class R, int M>
+__device__ __forceinline__ int collect_above(R &x, const float (&most)[M], uint32_t bound, Shared &sh, Hits *hits) {
   constexpr int N = R::N;
   uint4 *const chunks = reinterpret_cast<uint4 *>(sh.hist);
   uint32_t *const tags = reinterpret_cast<uint32_t *>(sh.cw);
@@ -228,24 +228,23 @@ __device__ __forceinline__ int collect_above(R &x, uint32_t bound, Shared &sh, H
   __syncthreads();
   const float least = value_of(bound);
   const bool every = least == kNegInf;
-  auto chunk = [&](const float (&v)[N], int i0, int n) -> bool {
-    float m = v[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
-    const bool hit = (m >= least || every) && n > 0;
-    if (hit) {
-      const int at = atomicAdd(&sh.above, 1);
-      if (at < kHitChunks) {
-        chunks[at] = R::E::pack(v);
-        tags[at] = uint32_t(n) << 24 | uint32_t(i0);
-      }
+  auto list = [&](const float (&v)[N], int i0, int n) {
+    const int at = atomicAdd(&sh.above, 1);
+    if (at < kHitChunks) {
+      chunks[at] = R::E::pack(v);
+      tags[at] = uint32_t(n) << 24 | uint32_t(i0);
     }
-    return hit;
   };
-  if constexpr (TAKE)
-    x.take(chunk);
-  else
-    x.each(chunk);
+  if constexpr (R::kResident) {
+    x.template above<TAKE>(most, least, every, list);
+  } else {
+    x.each([&](const float (&v)[N], int i0, int n) {
+      float m = v[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
+      if ((m >= least || every) && n > 0) list(v, i0, n);
+    });
+  }
   __syncthreads();
   *hits = {min(sh.above, kHitChunks), least, every};
   if (sh.above > kHitChunks) return kCand + 1;
@@ -561,11 +560,16 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
   const float u = P.uniforms[row];
   if (t < kTable) sh.table[t] = kPowers.v[t];
 
+  float most[NV > 0 ? NV : 1];  // of the chunks
   float mine = kNegInf;
-  x.each([&](const float (&v)[N], int, int) {
+  if constexpr (NV > 0) {
+    mine = x.maxima(most);
+  } else {
+    x.each([&](const float (&v)[N], int, int) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) mine = fmaxf(mine, v[i]);
-  });
+      for (int i = 0; i < N; ++i) mine = fmaxf(mine, v[i]);
+    });
+  }
   const float best = block_max<T>(mine, sh.red);
   auto answer = [&](int token, float logprob) {  // one thread
     P.tokens[row] = token;
@@ -606,7 +610,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
   const bool few = some && top_k <= T / 2;
   const uint32_t bound = bound_of<T>(mine, few ? top_k : kFirst, sh);
   Hits hits;
-  const int cnt = collect_above<T, false>(x, bound, sh, &hits);
+  const int cnt = collect_above<T, false>(x, most, bound, sh, &hits);
   const bool covers = few || cnt == V;  // no token past the list is kept
   // Whether min-p drops all tokens past the list, whose keys are below the bound.
   const bool m_in = min_p > 0.f && double(wt(value_of(bound))) < least;
@@ -740,15 +744,20 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
   const int V = int(L.vocab);
   R x;
   x.open(logits_row<DT>(L, row), V);
+  float most[NV > 0 ? NV : 1];  // of the chunks
   float mine = kNegInf;
-  x.each([&](const float (&v)[N], int, int) {
+  if constexpr (NV > 0) {
+    mine = x.maxima(most);
+  } else {
+    x.each([&](const float (&v)[N], int, int) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) mine = fmaxf(mine, v[i]);
-  });
+      for (int i = 0; i < N; ++i) mine = fmaxf(mine, v[i]);
+    });
+  }
   if (t == 0) s_next = 0;
   const uint32_t bound = bound_of<T>(mine, K, sh);
   Hits hits;
-  int cnt = collect_above<T, (NV > 0)>(x, bound, sh, &hits);
+  int cnt = collect_above<T, (NV > 0)>(x, most, bound, sh, &hits);
   const bool many = cnt > kCand;
   // Which tokens of the list are past the K-th.
   if (NV > 0 && !many)
@@ -837,8 +846,15 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
       auto term = [&](float v) { return __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -scaled)); };
       x.each([&](const float (&v)[N], int, int) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) z += term(fmaxf(v[i], kNegInf));
+        for (int i = 0; i < N; ++i) z += term(v[i]);
       });
+      if (__syncthreads_or(z != z)) {  // a NaN among the logits: once more, without it
+        z = 0.f;
+        x.each([&](const float (&v)[N], int, int) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) z += term(fmaxf(v[i], kNegInf));
+        });
+      }
       beside(term);
     } else {  // logits near the type's lowest value: subtracted before they are scaled
       ref2 = double(ref) * scale;
