@@ -739,7 +739,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
   using E = Elem<DT>;
   constexpr int N = R::N;
   __shared__ Shared sh;
-  __shared__ u64 s_last, s_next;
+  __shared__ u64 s_last, s_next, s_units;
   const int t = threadIdx.x, row = blockIdx.x;
   const int V = int(L.vocab);
   R x;
@@ -754,7 +754,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
       for (int i = 0; i < N; ++i) mine = fmaxf(mine, v[i]);
     });
   }
-  if (t == 0) s_next = 0;
+  if (t == 0) s_next = s_units = 0;
   const uint32_t bound = bound_of<T>(mine, K, sh);
   Hits hits;
   int cnt = collect_above<T, (NV > 0)>(x, most, bound, sh, &hits);
@@ -814,7 +814,8 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
   // The largest of the others: behind the K-th in the list, or below the list's bound.
   float m = next ? value_of(key_part(next)) : kNegInf;
   float z = 0.f;
-  double ref2;  // the sum's reference, in log2 units
+  double ref2 = 0.0;  // the sum's reference, in log2 units
+  bool done = false;
   if (NV > 0 && !many) {
     if (!next) {
       x.each([&](const float (&v)[N], int, int) {
@@ -826,10 +827,13 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
       });
       m = block_max<T>(m, sh.red);
     }
-    // What left the registers but is not among the K: the rest of those chunks,
-    // and of the list.  Both lists are in the order in which waves got there, so
-    // these terms (at most 1) are added up as whole multiples of 2^-40.
-    auto beside = [&](auto &&term) {
+    const float scaled = m == kNegInf ? 0.f : m * scale;
+    if (fabsf(scaled) < 1e30f) {
+      ref2 = double(scaled);
+      auto term = [&](float v) { return __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -scaled)); };
+      // What left the registers but is not among the K: the rest of those chunks,
+      // and of the list.  Both lists are in the order in which waves got there, so
+      // these terms (at most 1) are added up as whole multiples of 2^-40.
       u64 units = 0;
       auto add = [&](float v) { units += u64(term(v) * 1099511627776.f); };
       hits.template each<T, E>(sh, [&](float v, int, bool of_them) {
@@ -837,35 +841,25 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
       });
       for (int i = t; i < cnt; i += T)
         if (sh.fine[i]) add(value_of(key_part(sh.cand[i])));
-      units = block_add<T>(units, sh.scan);
-      if (t == 0) z += float(double(units) / 1099511627776.0);
-    };
-    const float ref = m == kNegInf ? 0.f : m, scaled = ref * scale;
-    if (fabsf(scaled) < 1e30f) {
-      ref2 = double(scaled);
-      auto term = [&](float v) { return __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -scaled)); };
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) units += __shfl_xor(units, o);
+      if ((t & 63) == 0) atomicAdd(&s_units, units);
       x.each([&](const float (&v)[N], int, int) {
 #pragma unroll
         for (int i = 0; i < N; ++i) z += term(v[i]);
       });
-      if (__syncthreads_or(z != z)) {  // a NaN among the logits: once more, without it
-        z = 0.f;
-        x.each([&](const float (&v)[N], int, int) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) z += term(fmaxf(v[i], kNegInf));
-        });
-      }
-      beside(term);
-    } else {  // logits near the type's lowest value: subtracted before they are scaled
-      ref2 = double(ref) * scale;
-      auto term = [&](float v) { return __builtin_amdgcn_exp2f((v - ref) * scale); };
-      x.each([&](const float (&v)[N], int, int) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) z += term(fmaxf(v[i], kNegInf));
-      });
-      beside(term);
+      z = wave_add(z);
+      __syncthreads();
+      if ((t & 63) == 0) sh.red[t >> 6] = z;
+      __syncthreads();
+      z = part_add<T / kWave>(sh.red) + float(double(s_units) / 1099511627776.0);
+      done = z == z;
     }
-  } else {
+  }
+  // Rows that are read again, too many equal logits, a NaN among them, or a
+  // largest other that overflows when it is scaled before it is subtracted.
+  if (!done) {
+    if (NV > 0 && !many) again.open(logits_row<DT>(L, row), V);
     const uint32_t kth = key_part(last);
     const float vk = value_of(kth);
     u64 in_list = 0;
@@ -881,22 +875,22 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
     }
     const float ref = m == kNegInf ? 0.f : m;
     ref2 = double(ref) * scale;
+    z = 0.f;
     again.each([&](const float (&v)[N], int, int) {
 #pragma unroll
       for (int i = 0; i < N; ++i) z += __builtin_amdgcn_exp2f(v[i] < vk ? (v[i] - ref) * scale : kNegInf);
     });
-    if (t == 0) z += ties;  // each of them is the reference itself: m = vk, exp = 1
+    z = wave_add(z);
+    __syncthreads();
+    if ((t & 63) == 0) sh.red[t >> 6] = z;
+    __syncthreads();
+    z = ties + part_add<T / kWave>(sh.red);  // each of the ties is the reference itself: m = vk, exp = 1
   }
-  z = wave_add(z);
-  __syncthreads();
-  if ((t & 63) == 0) sh.red[t >> 6] = z;
-  __syncthreads();
-  if (t < 16) {
-    z = part_add<T / kWave>(sh.red);
+  if (t == 0) {
     const double lse = m == kNegInf ? -__builtin_inf()
                        : m == __builtin_inff() ? __builtin_inf()
                                                : (ref2 + log2(double(z))) * 0.6931471805599453;
-    if (t == 0) rest[row] = float(lse);
+    rest[row] = float(lse);
   }
 }
 
