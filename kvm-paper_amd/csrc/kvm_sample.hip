@@ -49,6 +49,7 @@ typedef unsigned long long u64;
 constexpr int kBins = 2048;
 constexpr int kCand = 1024;        // tokens that are ranked by counting
 constexpr int kFirst = 128;        // tokens that sampling without a small top-k looks at first
+constexpr int kMany = 4096;        // tokens of the list for a larger top-k
 constexpr int kMaxTop = 512;       // K of the top logits
 constexpr double kUnit = 4398046511104.0;  // 2^42
 
@@ -412,7 +413,7 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
     x.template each<1>([&](const float (&v)[N], int i0, int n) {
       for (uint32_t bits = in_bin<Q, N>(wt, v, n, bin); bits; bits &= bits - 1) {
         const int idx = i0 + __ffs(bits) - 1;
-        const float xv = x.at(idx);
+        const float xv = N == 1 ? v[0] : x.at(idx);
         const uint32_t k = key_of(xv);
         if (k >= lo && k <= hi && (f_part < 0 || part_of(k) == f_part) && rank_of(k, idx) >= limit) f(k, idx, xv);
       }
@@ -520,8 +521,9 @@ __device__ __forceinline__ u64 build(const R &x, const Weights &wt, u64 limit, S
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const u64 w = Q == kCounted ? 1 : wt(v[i]);
-      if (i < n && wt.some(v[i]) && w && (limit == 0 || rank_of(key_of(v[i]), i0 + i) >= limit)) {
-        atomicAdd(&sh.hist[wt.bin(v[i])], w);
+      const float place = wt.place(v[i]);
+      if (i < n && place < float(kBins) && (limit == 0 || rank_of(key_of(v[i]), i0 + i) >= limit)) {
+        atomicAdd(&sh.hist[int(place)], w);
         if (Q == kWeighed && strong && double(w) >= least) big += w;
       }
     }
@@ -532,6 +534,75 @@ __device__ __forceinline__ u64 build(const R &x, const Weights &wt, u64 limit, S
 #pragma unroll
   for (int i = 0; i < PER; ++i) own += sh.hist[t * PER + i];
   return block_scan<T>(own, sh.scan, total);
+}
+
+// Tokens of a row in a list, as the functions above read a row.
+template <int T, class R>
+struct Listed {
+  static constexpr int N = 1;
+  const R &row;
+  const u64 *list;
+  int cnt;
+  __device__ __forceinline__ float at(int idx) const { return row.at(idx); }
+  template <int BATCH, class F>
+  __device__ __forceinline__ void each(F &&f) const {
+#pragma unroll 1
+    for (int i0 = 0; i0 < cnt; i0 += T) {
+      const int i = i0 + threadIdx.x;
+      const u64 token = list[min(i, cnt - 1)];
+      const float v[1] = {value_of(key_part(token))};
+      f(v, index_of(token), i < cnt ? 1 : 0);
+    }
+  }
+};
+
+// Lists the first tokens of the order, `want` or somewhat more (all that may
+// have a weight where there are fewer): a histogram of the chunks' maxima names
+// a bin whose edge `want` of them reach; the tokens before that edge are
+// collected.  Returns how many there are, kMany of them at most in the list.
+template <int T, class R>
+__device__ __forceinline__ int list_first(const R &x, const Weights &wt, int want, u64 *list, Shared &sh) {
+  constexpr int N = R::N, PER = kBins / T;
+  uint32_t *const hist = reinterpret_cast<uint32_t *>(sh.fine);
+  const int t = threadIdx.x;
+  __syncthreads();
+  for (int i = t; i < kBins; i += T) hist[i] = 0;
+  if (t == 0) {
+    sh.bin = kBins - 1;
+    sh.count = 0;
+  }
+  __syncthreads();
+  x.template each<1>([&](const float (&v)[N], int, int) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
+    if (wt.some(m)) atomicAdd(&hist[wt.bin(m)], 1u);
+  });
+  __syncthreads();
+  uint32_t own = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) own += hist[t * PER + i];
+  u64 all;
+  int s = int(block_scan<T>(own, sh.scan, &all));
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int q = int(hist[t * PER + i]);
+    if (s < want && s + q >= want) sh.bin = t * PER + i;
+    s += q;
+  }
+  __syncthreads();
+  const float edge = float(sh.bin + 1);
+  x.template each<1>([&](const float (&v)[N], int i0, int n) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (wt.place(v[i]) < edge && i < n) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kMany) list[at] = rank_of(key_of(v[i]), i0 + i);
+      }
+    }
+  });
+  __syncthreads();
+  return sh.count;
 }
 
 // floor(u * c) for a uniform number, inside [0, c - 1] whatever u is.
@@ -547,6 +618,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
   using R = Row<DT, T, NV, true>;
   constexpr int N = R::N;
   __shared__ Shared sh;
+  __shared__ u64 many[NV == 0 ? kMany : 1];
   const int t = threadIdx.x, row = blockIdx.x;
   const int V = int(P.logits.vocab);
   R x;
@@ -620,7 +692,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
       sorted[r] = me;
       weight[r] = wt(value_of(key_part(me)));
     });
-    u64 z = 0, strong = 0;
+    u64 z = 0, strong = 0;  // the weight of the row, and of its tokens that min-p keeps
     // The weight of the row, unless min-p alone says where the kept tokens end.
     if (!covers && !(m_in && top_p >= 1.f)) {
       if (best == __builtin_inff()) {
@@ -666,8 +738,8 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
       }
       const u64 sum = __shfl(before, kWave - 1);
       before -= own;
-      if (covers) z = sum;
-      const double end = double(top_p) * double(z);
+      const u64 whole = covers ? sum : z;
+      const double end = double(top_p) * double(whole);
       // What is kept of the list: each lane's last kept running sum, the largest of them.
       u64 c = 0, run = before;
       for (int i = first; i < last; ++i) {
@@ -703,33 +775,46 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
     __syncthreads();
     if (sh.count) return;
   }
-  u64 limit = 0;  // the last token that top-k keeps (0: it keeps all)
-  u64 z;
-  if (some) {
-    const u64 pre = build<T, kCounted>(again, wt, 0, sh, &z, 0.0, nullptr);
-    if (u64(top_k) < z) {
-      locate<T, kCounted>(again, wt, u64(top_k) - 1, pre, 0, sh);
-      limit = sh.found;
+  // The draw, by locating, among the tokens of the row, or of a list that holds
+  // all that top-k keeps.
+  auto draw = [&](const auto &tokens) {
+    u64 limit = 0, total;  // limit: the last token that top-k keeps (0: it keeps all)
+    if (some) {
+      const u64 pre = build<T, kCounted>(tokens, wt, 0, sh, &total, 0.0, nullptr);
+      if (u64(top_k) < total) {
+        locate<T, kCounted>(tokens, wt, u64(top_k) - 1, pre, 0, sh);
+        limit = sh.found;
+      }
     }
-  }
-  u64 strong = 0;
-  const u64 pre = build<T, kWeighed>(again, wt, limit, sh, &z, least, min_p > 0.f ? &strong : nullptr);
-  u64 c = z;
+    u64 kept_strong = 0;
+    const u64 pre = build<T, kWeighed>(tokens, wt, limit, sh, &total, least, min_p > 0.f ? &kept_strong : nullptr);
+    u64 c = total;
 #pragma unroll 1
-  for (int step = top_p < 1.f ? 0 : 1; step < 2; ++step) {  // where top-p ends, then the draw
-    u64 target;
-    if (step == 0) {
-      const double end = ceil(double(top_p) * double(z));
-      target = end >= 1.0 ? u64(end) - 1 : 0;
-    } else {
-      if (min_p > 0.f && strong < c) c = strong;
-      if (c < u64(kUnit)) c = u64(kUnit);  // the first token is always kept
-      target = target_of(u, c);
+    for (int step = top_p < 1.f ? 0 : 1; step < 2; ++step) {  // where top-p ends, then the draw
+      u64 target;
+      if (step == 0) {
+        const double end = ceil(double(top_p) * double(c));
+        target = end >= 1.0 ? u64(end) - 1 : 0;
+      } else {
+        if (min_p > 0.f && kept_strong < c) c = kept_strong;
+        if (c < u64(kUnit)) c = u64(kUnit);  // the first token is always kept
+        target = target_of(u, c);
+      }
+      locate<T, kWeighed>(tokens, wt, target, pre, limit, sh);
+      if (step == 0) c = sh.found_end;
     }
-    locate<T, kWeighed>(again, wt, target, pre, limit, sh);
-    if (step == 0) c = sh.found_end;
+    if (t == 0) write(sh.found, c);
+  };
+  if constexpr (NV == 0) {
+    if (some && top_k <= kMany / 2) {
+      const int listed = list_first<T>(again, wt, top_k, many, sh);
+      if (listed <= kMany) {
+        draw(Listed<T, Row<DT, T, 0>>{again, many, listed});
+        return;
+      }
+    }
   }
-  if (t == 0) write(sh.found, c);
+  draw(again);
 }
 
 template <int DT, int T, int NV>

@@ -100,6 +100,14 @@ def test_sample_short_rows_and_many_rows(V, n, kw):
     _check_sample(_logits(n, V, torch.bfloat16, V, 1.0), torch.rand(n, generator=_gen(V + n)), "short", **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(top_p=0.9), dict(top_p=0.6, min_p=0.001), dict(top_k=1500, top_p=0.97),
+                                dict(top_k=2000, min_p=0.005), dict(), dict(top_k=2040)])
+@pytest.mark.parametrize("spread", [0.02, 0.5, 1.0])
+def test_sample_flat_rows(spread, kw):
+    """Distributions whose nucleus is hundreds or thousands of tokens."""
+    _check_sample(_logits(6, 20011, torch.float32, 77, spread), torch.rand(6, generator=_gen(78)), "flat", **kw)
+
+
 def test_sample_settings_per_row():
     n = 24
     g = _gen(9)
