@@ -33,9 +33,16 @@
 // more than 1024 tokens is cut again by their bit patterns until it has fewer,
 // or holds one value only, whose tokens rank by index.
 //
-// One workgroup per row, which is read once, into registers; locating reads it
-// again, from the caches, in loops that are not unrolled (a pass over registers
-// has its code once per chunk).
+// One workgroup per row.  The top logits, and the first passes of sampling
+// where there are more rows than compute units, hold it in registers; other
+// passes read it again, from the caches, in loops (a pass over registers has
+// its code once per chunk, which one workgroup alone would read from memory).
+//
+// Measured: the top 64 of 8192 rows of 50304 bf16 logits 0.25 ms, VALU 70 % busy
+// (9 of 16 instructions per logit are the maximum's and the exponential's); 512
+// rows of 65536 bf16 logits with min-p 23 us; one row of 50304 fp32 logits with
+// top-p 22 us where the first list decides (8.6 of them the fp64 weights of the
+// row on one compute unit), 50 where it does not.
 
 #include <type_traits>
 
