@@ -64,6 +64,12 @@ int check_layer(const kvm_layer *L) {
   return KVM_OK;
 }
 
+// A number whose fp32 value and its reciprocal are positive and finite.
+bool positive_f32(double v) {
+  const float f = float(v);
+  return f > 0.f && std::isfinite(f) && std::isfinite(2.f / f);
+}
+
 int check_logits(const kvm_logits *L, const char *what) {
   if (!L || !L->data) return fail(KVM_EINVAL, "%s: logits must be set", what);
   if (L->dtype < KVM_BF16 || L->dtype > KVM_F32) return fail(KVM_EINVAL, "%s: unknown logits type", what);
@@ -258,8 +264,8 @@ int kvm_top_logits(const kvm_logits *logits, int64_t k, double temperature, void
   if (k < 1 || k > logits->vocab || k > kvm::top_logits_max())
     return fail(KVM_EINVAL, "top_logits: k must be in [1, min(vocab, %lld)], got %lld",
                 (long long)kvm::top_logits_max(), (long long)k);
-  if (!(temperature > 0.0) || !std::isfinite(temperature))
-    return fail(KVM_EINVAL, "top_logits: temperature must be positive and finite");
+  if (!positive_f32(temperature))
+    return fail(KVM_EINVAL, "top_logits: temperature must be positive and finite in fp32");
   if (!values || !indices) return fail(KVM_EINVAL, "top_logits: values and indices must be set");
   KVM_HIP(kvm::launch_top_logits(*logits, k, temperature, values, indices, rest, as_stream(stream)), "top_logits");
   return KVM_OK;
@@ -293,8 +299,8 @@ int kvm_head_loss(const kvm_head_loss_desc *d, void *stream) {
   if (P.k > 0) {
     if (!P.t_values || !P.t_indices) return fail(KVM_EINVAL, "head_loss: teacher values and indices must be set");
     if (P.t_dtype < KVM_BF16 || P.t_dtype > KVM_F32) return fail(KVM_EINVAL, "head_loss: unknown teacher type");
-    if (!(P.temperature > 0.0) || !std::isfinite(P.temperature))
-      return fail(KVM_EINVAL, "head_loss: temperature must be positive and finite");
+    if (!positive_f32(P.temperature))
+      return fail(KVM_EINVAL, "head_loss: temperature must be positive and finite in fp32");
     if (!(P.label_weight >= 0.0 && P.label_weight <= 1.0))
       return fail(KVM_EINVAL, "head_loss: label_weight must be in [0, 1]");
     if (P.label_weight > 0.0 && !P.labels) return fail(KVM_EINVAL, "head_loss: label_weight needs labels");

@@ -140,6 +140,7 @@ struct Shared {
   int ired[16];
   uint32_t kmin, kmax;
   int count, bin;
+  int hit_chunks, hit_tokens;
   u64 base;        // weight (or count) before the located bin
   u64 found;       // the located token (its rank_of)
   u64 found_end;   // running sum including it
@@ -232,12 +233,12 @@ __device__ __forceinline__ int collect_above(R &x, const float (&most)[M], uint3
   constexpr int N = R::N;
   uint4 *const chunks = reinterpret_cast<uint4 *>(sh.hist);
   uint32_t *const tags = reinterpret_cast<uint32_t *>(sh.cw);
-  if (threadIdx.x == 0) sh.count = sh.above = 0;
+  if (threadIdx.x == 0) sh.hit_chunks = sh.hit_tokens = 0;
   __syncthreads();
   const float least = value_of(bound);
   const bool every = least == kNegInf;
   auto list = [&](const float (&v)[N], int i0, int n) {
-    const int at = atomicAdd(&sh.above, 1);
+    const int at = atomicAdd(&sh.hit_chunks, 1);
     if (at < kHitChunks) {
       chunks[at] = R::E::pack(v);
       tags[at] = uint32_t(n) << 24 | uint32_t(i0);
@@ -254,16 +255,16 @@ __device__ __forceinline__ int collect_above(R &x, const float (&most)[M], uint3
     });
   }
   __syncthreads();
-  *hits = {min(sh.above, kHitChunks), least, every};
-  if (sh.above > kHitChunks) return kCand + 1;
+  *hits = {min(sh.hit_chunks, kHitChunks), least, every};
+  if (sh.hit_chunks > kHitChunks) return kCand + 1;
   hits->template each<T, typename R::E>(sh, [&](float v, int idx, bool of_them) {
     if (of_them) {
-      const int at = atomicAdd(&sh.count, 1);
+      const int at = atomicAdd(&sh.hit_tokens, 1);
       if (at < kCand) sh.cand[at] = rank_of(key_of(v), idx);
     }
   });
   __syncthreads();
-  return sh.count;
+  return sh.hit_tokens;
 }
 
 // Inclusive prefix sum over a wave: shifts within rows of 16 lanes, then the
@@ -851,9 +852,6 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
   Hits hits;
   int cnt = collect_above<T, (NV > 0)>(x, most, bound, sh, &hits);
   const bool many = cnt > kCand;
-  // Which tokens of the list are past the K-th.
-  if (NV > 0 && !many)
-    for (int i = t; i < cnt; i += T) sh.fine[i] = 0;
   Row<DT, T, 0> again;  // for rows that are not in registers, or no longer whole there
   if (NV == 0 || many) again.open(logits_row<DT>(L, row), V);
   u64 more_ties = 0;  // tokens of the K-th value behind it that are not in the list
@@ -891,8 +889,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
     more_ties = block_add<T>(ties, sh.scan);
     cnt = K;
   }
-  ranked<T>(cnt, sh, [&](int i, u64 me, int r) {
-    if (NV > 0 && !many && r >= K) sh.fine[i] = 1;
+  ranked<T>(cnt, sh, [&](int, u64 me, int r) {
     if (r < K) {
       static_cast<typename E::raw *>(values)[int64_t(row) * K + r] = E::put(value_of(key_part(me)));
       indices[int64_t(row) * K + r] = index_of(me);
@@ -932,7 +929,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
         if (!of_them) add(fmaxf(v, kNegInf));
       });
       for (int i = t; i < cnt; i += T)
-        if (sh.fine[i]) add(value_of(key_part(sh.cand[i])));
+        if (sh.cand[i] < last) add(value_of(key_part(sh.cand[i])));
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) units += __shfl_xor(units, o);
       if ((t & 63) == 0) atomicAdd(&s_units, units);

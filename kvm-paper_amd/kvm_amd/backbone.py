@@ -30,6 +30,7 @@ as given.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import importlib
 import math
@@ -653,15 +654,30 @@ class RWKV7BackboneForCausalLM(nn.Module):
         B, T = input_ids.shape
         cache = StatesDictCache() if cache is None else cache
         u = _uniforms(uniforms, input_ids, max_new_tokens, generator)
-        logits = self(input_ids=input_ids, past_key_values=cache, use_cache=True,
-                      cache_position=torch.arange(T, device=input_ids.device), logits_to_keep=1).logits[:, -1]
 
         def step(tok, s):
             return self(input_ids=tok[:, None], past_key_values=cache, use_cache=True,
                         cache_position=torch.tensor([T + s], device=input_ids.device), logits_to_keep=1).logits[:, -1]
 
         settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-        return _sample_loop(logits, step, u, settings, return_logprobs)
+        with _evaluating(self):
+            logits = self(input_ids=input_ids, past_key_values=cache, use_cache=True,
+                          cache_position=torch.arange(T, device=input_ids.device), logits_to_keep=1).logits[:, -1]
+            return _sample_loop(logits, step, u, settings, return_logprobs)
+
+
+@contextlib.contextmanager
+def _evaluating(model: nn.Module):
+    """``model`` in evaluation mode, each module as it was afterwards: cached
+    decoding is the inference path, also for a model that is being trained."""
+    training = [m for m in model.modules() if m.training]
+    for m in training:
+        m.training = False
+    try:
+        yield
+    finally:
+        for m in training:
+            m.training = True
 
 
 def _uniforms(uniforms, input_ids, n, generator):
@@ -839,10 +855,11 @@ class DecodeGraph:
         """``RWKV7BackboneForCausalLM.generate_sampled`` through this runner."""
         B, T = input_ids.shape
         u = _uniforms(uniforms, input_ids, max_new_tokens, generator)
-        logits = self.model(input_ids=input_ids, past_key_values=self.cache, use_cache=True,
-                            cache_position=torch.arange(T, device=input_ids.device), logits_to_keep=1).logits[:, -1]
         settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-        return _sample_loop(logits, lambda tok, s: self.step(tok), u, settings, return_logprobs)
+        with _evaluating(self.model):
+            logits = self.model(input_ids=input_ids, past_key_values=self.cache, use_cache=True,
+                                cache_position=torch.arange(T, device=input_ids.device), logits_to_keep=1).logits[:, -1]
+            return _sample_loop(logits, lambda tok, s: self.step(tok), u, settings, return_logprobs)
 
 
 @torch.no_grad()

@@ -153,6 +153,17 @@ def test_sample_large_vocabulary_and_ties():
         _check_sample(x, torch.rand(3, generator=_gen(2)), "large", **kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_largest_vocabulary(dtype):
+    V = 1 << 20
+    x = _logits(2, V, dtype, 35, 1.5)
+    x[1] = x[1].clamp(max=1.0)                     # a tenth of the tokens equal the largest
+    for kw in (dict(top_p=0.9), dict(top_k=100), dict()):
+        _check_sample(x, torch.tensor([0.3, 0.999]), "largest", **kw)
+    _check_top(x, 512, 1.0, "largest")
+    _check_loss(x, torch.tensor([V - 1, 5]), _teacher(2, V, 1024, 36, dtype), 0.5, "largest")
+
+
 def test_sample_views_and_shapes():
     import kvm_amd as K
 
@@ -230,6 +241,7 @@ def test_top_logits_degenerate_rows(dtype, k):
     x[10, ::7] = 0.0
     x[6, 0::9] = torch.finfo(dtype).min
     x[0, :3000] = torch.finfo(dtype).min           # with k = 500: equal lowest values, the others nothing
+    x[4, ::2] = torch.arange(V)[::2].remainder(100) * 2.0 ** -133  # subnormal, in order all the same
     _check_top(x, k, 1.0, "degenerate")
 
 
@@ -253,8 +265,9 @@ def test_top_logits_views_streams_and_refusals():
     for k in (0, 513, 2004):
         with pytest.raises(ValueError, match="k must be"):
             K.top_logits(base, k)
-    with pytest.raises(ValueError, match="temperature"):
-        K.top_logits(base, 3, temperature=0.0)
+    for bad in (0.0, -1.0, math.inf, math.nan, 1e-50, 1e-39):
+        with pytest.raises(ValueError, match="temperature"):
+            K.top_logits(base, 3, temperature=bad)
 
 
 # ---------------------------------------------------------------- losses
@@ -403,7 +416,8 @@ def test_loss_views(dtype):
     base = _logits(4 * 6, 517, dtype, 100).view(4, 6, 517).to(DEV)
     labels = torch.randint(0, 400, (4, 6), generator=_gen(101)).to(DEV)
     for cut in (lambda t: t[:, :-1], lambda t: t[..., 1:], lambda t: t[:, 1:, 2:500], lambda t: t[::2, 3],
-                lambda t: t.transpose(0, 1), lambda t: t[1, 2], lambda t: t[:, ::2]):
+                lambda t: t.transpose(0, 1), lambda t: t[1, 2], lambda t: t[:, ::2],
+                lambda t: t.transpose(0, 2).contiguous().transpose(0, 2)):  # the vocabulary not contiguous: a copy
         view = cut(base)
         lab = cut(labels.unsqueeze(-1).expand(4, 6, 517))[..., 0].contiguous()
         a = view.detach().requires_grad_(True)
@@ -591,6 +605,10 @@ def test_on_policy_distillation_step(softcap):
     student, teacher = _model(2, softcap).train(), _model(3, softcap).eval()
     prompt = torch.randint(0, 515, (2, 100), generator=_gen(210)).to(DEV)
     rollout = student.generate_sampled(prompt, 29, top_p=0.9, generator=torch.Generator(device=DEV).manual_seed(1))
+    assert student.training and all(m.training for m in student.modules())
+    again = _model(2, softcap).eval().generate_sampled(prompt, 29, top_p=0.9,
+                                                       generator=torch.Generator(device=DEV).manual_seed(1))
+    assert torch.equal(rollout, again)  # a model in training samples as it does in evaluation
     ids = torch.cat([prompt, rollout], 1)
     labels = ids.clone()
     labels[:, :100] = -100                         # the prompt is not learnt
