@@ -375,9 +375,9 @@ __device__ __forceinline__ uint32_t in_bin(const Weights &wt, const float (&v)[N
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const float p = wt.place(v[i]);
-    bits |= (Q == kEvery || (p >= float(bin) && p < float(bin + 1))) && i < n ? 1u << i : 0u;
+    bits |= Q == kEvery || (p >= float(bin) && p < float(bin + 1)) ? 1u << i : 0u;
   }
-  return bits;
+  return bits & ((1u << n) - 1);
 }
 
 // The token at running sum `target` (before <= target < before + its own) in
@@ -420,8 +420,10 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
   auto tokens = [&](auto &&f) {  // f(key, index, value) for each of them
     x.template each<1>([&](const float (&v)[N], int i0, int n) {
       for (uint32_t bits = in_bin<Q, N>(wt, v, n, bin); bits; bits &= bits - 1) {
-        const int idx = i0 + __ffs(bits) - 1;
-        const float xv = N == 1 ? v[0] : x.at(idx);
+        const int e = __ffs(bits) - 1, idx = i0 + e;
+        float xv = v[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) xv = e == i ? v[i] : xv;
         const uint32_t k = key_of(xv);
         if (k >= lo && k <= hi && (f_part < 0 || part_of(k) == f_part) && rank_of(k, idx) >= limit) f(k, idx, xv);
       }
@@ -456,8 +458,10 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
         const u64 me = sh.cand[i];
         u64 before = 0;
 #pragma unroll 4
-        for (int j = part; j < cnt; j += lanes)
-          if (sh.cand[j] > me) before += sh.cw[j];
+        for (int j = part; j < cnt; j += lanes) {
+          const u64 w = sh.cw[j];
+          before += sh.cand[j] > me ? w : 0;
+        }
         for (int o = lanes / 2; o >= 1; o >>= 1) before += __shfl_xor(before, o);
         before += base;
         if (target >= before && target < before + sh.cw[i]) {
@@ -525,17 +529,25 @@ __device__ __forceinline__ u64 build(const R &x, const Weights &wt, u64 limit, S
   for (int i = t; i < kBins; i += T) sh.hist[i] = 0;
   __syncthreads();
   u64 big = 0;
-  x.template each<1>([&](const float (&v)[N], int i0, int n) {
+  auto pass = [&](auto &&weight) {
+    x.template each<1>([&](const float (&v)[N], int i0, int n) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const u64 w = Q == kCounted ? 1 : wt(v[i]);
-      const float place = wt.place(v[i]);
-      if (i < n && place < float(kBins) && (limit == 0 || rank_of(key_of(v[i]), i0 + i) >= limit)) {
-        atomicAdd(&sh.hist[int(place)], w);
-        if (Q == kWeighed && strong && double(w) >= least) big += w;
+      for (int i = 0; i < N; ++i) {
+        const u64 w = weight(v[i]);
+        const float place = wt.place(v[i]);
+        if (i < n && place < float(kBins) && (limit == 0 || rank_of(key_of(v[i]), i0 + i) >= limit)) {
+          atomicAdd(&sh.hist[int(place)], w);
+          if (Q == kWeighed && strong && double(w) >= least) big += w;
+        }
       }
-    }
-  });
+    });
+  };
+  if constexpr (Q == kCounted)
+    pass([](float) { return u64(1); });
+  else if (wt.best == __builtin_inff())
+    pass([&](float v) { return u64(v == wt.best ? kUnit : 0.0); });
+  else
+    pass([&](float v) { return __builtin_bit_cast(u64, wt.raised(v)) & 0xfffffffffffffull; });
   __syncthreads();
   if (Q == kWeighed && strong) *strong = block_add<T>(big, sh.scan);
   u64 own = 0;
@@ -545,13 +557,11 @@ __device__ __forceinline__ u64 build(const R &x, const Weights &wt, u64 limit, S
 }
 
 // Tokens of a row in a list, as the functions above read a row.
-template <int T, class R>
+template <int T>
 struct Listed {
   static constexpr int N = 1;
-  const R &row;
   const u64 *list;
   int cnt;
-  __device__ __forceinline__ float at(int idx) const { return row.at(idx); }
   template <int BATCH, class F>
   __device__ __forceinline__ void each(F &&f) const {
 #pragma unroll 1
@@ -817,7 +827,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
     if (some && top_k <= kMany / 2) {
       const int listed = list_first<T>(again, wt, top_k, many, sh);
       if (listed <= kMany) {
-        draw(Listed<T, Row<DT, T, 0>>{again, many, listed});
+        draw(Listed<T>{many, listed});
         return;
       }
     }
