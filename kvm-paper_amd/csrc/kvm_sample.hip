@@ -22,9 +22,11 @@
 // pass (T ln(1 / (1 - k/T)) of them for T threads and logits in no particular
 // order); those that do are collected and ranked by counting, each against
 // each.  That is all that the top logits and a small top-k need.  Without one,
-// sampling adds up the weights of the whole row, and is done where the tokens
-// so ranked hold what top-p asks for and the draw falls on one of them, as it
-// does unless a distribution is rather flat.
+// sampling is done where the tokens so ranked hold what top-p asks for and the
+// draw falls on one of them, as it does unless a distribution is rather flat.
+// For top-p that takes the weight of the whole row only as closely as to tell
+// which token it ends on: a sum in fp32 with its error bound, and the exact one
+// where a token's edge falls within that bound or C is the weight of the row.
 //
 // Locating, in general: a histogram of weights (or counts) over 2048 bins that
 // are linear in (x_0 - x) / T up to the 43 ln 2 past which weights are zero; a
@@ -41,8 +43,8 @@
 // Measured: the top 64 of 8192 rows of 50304 bf16 logits 0.25 ms, VALU 70 % busy
 // (9 of 16 instructions per logit are the maximum's and the exponential's); 512
 // rows of 65536 bf16 logits with min-p 23 us; one row of 50304 fp32 logits with
-// top-p 22 us where the first list decides (8.6 of them the fp64 weights of the
-// row on one compute unit), 50 where it does not.
+// top-p 16 us where the first list decides (22 with the exact weight of the row
+// on one compute unit), 50 where it does not.
 
 #include <type_traits>
 
@@ -228,8 +230,11 @@ constexpr int kHitChunks = 1024;
 // than kCand where their chunks do not fit either).  A pass over a row has its
 // code once per chunk, so a chunk with such a token only goes to LDS; its
 // tokens are looked at from there.  TAKE: those chunks leave the registers.
-template <int T, bool TAKE, class R, int M>
-__device__ __forceinline__ int collect_above(R &x, const float (&most)[M], uint32_t bound, Shared &sh, Hits *hits) {
+// also(v) is called on the way for the values of every chunk of a row that is
+// read again, also(x) for a row in registers.
+template <int T, bool TAKE, class R, int M, class F>
+__device__ __forceinline__ int collect_above(R &x, const float (&most)[M], uint32_t bound, Shared &sh, Hits *hits,
+                                             F &&also) {
   constexpr int N = R::N;
   uint4 *const chunks = reinterpret_cast<uint4 *>(sh.hist);
   uint32_t *const tags = reinterpret_cast<uint32_t *>(sh.cw);
@@ -246,8 +251,10 @@ __device__ __forceinline__ int collect_above(R &x, const float (&most)[M], uint3
   };
   if constexpr (R::kResident) {
     x.template above<TAKE>(most, least, every, list);
+    also(x);
   } else {
     x.each([&](const float (&v)[N], int i0, int n) {
+      also(v);
       float m = v[0];
 #pragma unroll
       for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
@@ -699,20 +706,108 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
   const bool some = top_k > 0 && top_k < V;  // top-k drops tokens
   const bool few = some && top_k <= T / 2;
   const uint32_t bound = bound_of<T>(mine, few ? top_k : kFirst, sh);
-  Hits hits;
-  const int cnt = collect_above<T, false>(x, most, bound, sh, &hits);
-  const bool covers = few || cnt == V;  // no token past the list is kept
   // Whether min-p drops all tokens past the list, whose keys are below the bound.
   const bool m_in = min_p > 0.f && double(wt(value_of(bound))) < least;
+  // Whether the row's weight matters: not where top-k or min-p alone says where the kept tokens end.
+  const bool weighed = !some && !(m_in && top_p >= 1.f);
+  // That weight in fp32, on the way: enough to tell where top-p ends unless
+  // that falls on the edge of a token within its error.
+  float about = 0.f;
+  const float log2_per = 1.4426950408889634f / temp;
+  auto terms = [&](const float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) about += __builtin_amdgcn_exp2f((v[i] - best) * log2_per);
+  };
+  Hits hits;
+  const int cnt = collect_above<T, false>(x, most, bound, sh, &hits, [&](const auto &part) {
+    if constexpr (NV > 0) {
+      if (weighed) part.each([&](const float (&v)[N], int, int) { terms(v); });
+    } else {
+      if (weighed) terms(part);
+    }
+  });
+  const bool covers = few || cnt == V;  // no token past the list is kept
   if (cnt <= kCand && (covers || !some)) {
     u64 *sorted = sh.hist, *weight = sh.hist + kCand;
     ranked<T>(cnt, sh, [&](int, u64 me, int r) {
       sorted[r] = me;
       weight[r] = wt(value_of(key_part(me)));
     });
-    u64 z = 0, strong = 0;  // the weight of the row, and of its tokens that min-p keeps
-    // The weight of the row, unless min-p alone says where the kept tokens end.
-    if (!covers && !(m_in && top_p >= 1.f)) {
+    about = wave_add(about);
+    if ((t & 63) == 0) sh.red[t >> 6] = about;
+    __syncthreads();
+    enum { kDone, kWeigh, kLocate };
+    // One wave finishes: consecutive tokens per lane, a prefix sum of their
+    // weights.  The row's weight is within [z_lo, z_hi]; where they are equal, z
+    // and strong (the weight of its tokens that min-p keeps) are exact.  Leaves in
+    // sh.count whether the token was found, needs the exact weight, or lies past
+    // the list.
+    auto finish = [&](double z_lo, double z_hi, u64 z, u64 strong) {
+      if (t < kWave) {
+        const int k = some ? min(top_k, cnt) : cnt, per = (k + kWave - 1) / kWave;
+        const int first = min(t * per, k), last = min(first + per, k);
+        u64 own = 0;
+        for (int i = first; i < last; ++i) own += weight[i];
+        u64 before = own;
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+          const u64 up = __shfl_up(before, o);
+          if (t >= o) before += up;
+        }
+        const u64 sum = __shfl(before, kWave - 1);
+        before -= own;
+        if (covers) z_lo = z_hi = double(sum);
+        const bool exact = z_lo == z_hi;
+        const double end_lo = double(top_p) * z_lo, end_hi = double(top_p) * z_hi;
+        // What is kept of the list: each lane's last kept running sum, the largest of them.
+        u64 c = 0, run = before;
+        bool edge = false;  // a token that top-p may keep or not
+        for (int i = first; i < last; ++i) {
+          const u64 w = weight[i];
+          const double at = double(run);
+          if (i == 0 || ((top_p >= 1.f || at < end_lo) && double(w) >= least)) c = run + w;
+          edge = edge || (i > 0 && top_p < 1.f && at >= end_lo && at < end_hi);
+          run += w;
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+          const u64 other = __shfl_xor(c, o);
+          c = other > c ? other : c;
+        }
+        int state = __ballot(edge) ? kWeigh : kDone;
+        if (!covers && !m_in) {
+          if (top_p >= 1.f) {  // past the list: the weight of the row, or of what min-p keeps of it
+            c = min_p > 0.f ? strong : z;
+            if (!exact) state = min_p <= 0.f && double(u) * z_lo > double(sum) ? kLocate : kWeigh;
+          } else if (double(sum) < end_hi) {  // top-p may end past the list
+            state = double(sum) < end_lo ? kLocate : kWeigh;
+          }
+        }
+        if (!(z_lo <= z_hi)) state = kWeigh;  // NaN: infinities or NaN among the logits
+        if (state == kDone) {
+          const u64 at = target_of(u, c);
+          if (at >= sum) state = kLocate;
+          run = before;
+          for (int i = first; i < last; ++i) {
+            const u64 w = weight[i];
+            if (at >= run && at < run + w) write(sorted[i], c);
+            run += w;
+          }
+        }
+        if (t == 0) sh.count = state;
+      }
+      __syncthreads();
+      return sh.count;
+    };
+    // The fp32 sum is off by at most 2^-24 of it for every term a thread adds,
+    // and 2^-17 for the exponentials' arguments (three roundings of at most 62
+    // octaves); the weights' own roundings and the terms below their unit are
+    // 2^-22 at most.  Both are taken with a margin, 2^-22 a term and 2^-16.
+    const double sum32 = weighed ? double(part_add<T / kWave>(sh.red)) * kUnit : 0.0;
+    const double off = sum32 * (double(V / T + 64) / 4194304.0);
+    int state = finish(sum32 - off, sum32 + off, 0, 0);
+    if (state == kWeigh) {
+      u64 z = 0, strong = 0;
       if (best == __builtin_inff()) {
         again.template each<1>([&](const float (&v)[N], int, int) {
 #pragma unroll
@@ -740,58 +835,9 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_s
         strong = block_add<T>(strong, sh.scan);
       }
       z = block_add<T>(z, sh.scan);
+      state = finish(double(z), double(z), z, strong);
     }
-    __syncthreads();
-    bool done = true;
-    if (t < kWave) {  // one wave finishes: consecutive tokens per lane, a prefix sum of their weights
-      const int k = some ? min(top_k, cnt) : cnt, per = (k + kWave - 1) / kWave;
-      const int first = min(t * per, k), last = min(first + per, k);
-      u64 own = 0;
-      for (int i = first; i < last; ++i) own += weight[i];
-      u64 before = own;
-#pragma unroll
-      for (int o = 1; o < kWave; o <<= 1) {
-        const u64 up = __shfl_up(before, o);
-        if (t >= o) before += up;
-      }
-      const u64 sum = __shfl(before, kWave - 1);
-      before -= own;
-      const u64 whole = covers ? sum : z;
-      const double end = double(top_p) * double(whole);
-      // What is kept of the list: each lane's last kept running sum, the largest of them.
-      u64 c = 0, run = before;
-      for (int i = first; i < last; ++i) {
-        const u64 w = weight[i];
-        if (i == 0 || ((top_p >= 1.f || double(run) < end) && double(w) >= least)) c = run + w;
-        run += w;
-      }
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) {
-        const u64 other = __shfl_xor(c, o);
-        c = other > c ? other : c;
-      }
-      if (!covers) {
-        // Past the list: the weight of the row, unless top-p or min-p ends inside it.
-        const bool p_in = top_p < 1.f && double(sum) >= end;
-        if (!p_in && !m_in) {
-          done = top_p >= 1.f;
-          c = min_p > 0.f ? strong : z;
-        }
-      }
-      const u64 at = target_of(u, c);
-      done = done && at < sum;
-      if (done) {
-        run = before;
-        for (int i = first; i < last; ++i) {
-          const u64 w = weight[i];
-          if (at >= run && at < run + w) write(sorted[i], c);
-          run += w;
-        }
-      }
-      if (t == 0) sh.count = done;
-    }
-    __syncthreads();
-    if (sh.count) return;
+    if (state == kDone) return;
   }
   // The draw, by locating, among the tokens of the row, or of a list that holds
   // all that top-k keeps.
@@ -860,7 +906,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_t
   if (t == 0) s_next = s_units = 0;
   const uint32_t bound = bound_of<T>(mine, K, sh);
   Hits hits;
-  int cnt = collect_above<T, (NV > 0)>(x, most, bound, sh, &hits);
+  int cnt = collect_above<T, (NV > 0)>(x, most, bound, sh, &hits, [](const auto &) {});
   const bool many = cnt > kCand;
   Row<DT, T, 0> again;  // for rows that are not in registers, or no longer whole there
   if (NV == 0 || many) again.open(logits_row<DT>(L, row), V);

@@ -108,6 +108,31 @@ def test_sample_flat_rows(spread, kw):
     _check_sample(_logits(6, 20011, torch.float32, 77, spread), torch.rand(6, generator=_gen(78)), "flat", **kw)
 
 
+@pytest.mark.parametrize("n", [9, 270])
+@pytest.mark.parametrize("min_p", [0.0, 1e-3])
+def test_nucleus_that_ends_on_the_edge_of_a_token(n, min_p):
+    """top_p at the running sum of some tokens over the weight of the row, and
+    the fp32 numbers beside it: a sum in fp32 does not tell them apart."""
+    x = _logits(n, 6007, torch.float32, 79, 3.0)
+    w = torch.exp((x.double() - x.max(1, keepdim=True).values.double())).sort(dim=1, descending=True).values
+    share = w.cumsum(1) / w.sum(1, keepdim=True)
+    p = torch.stack([share[i, (3 * i) % 40] for i in range(n)]).float()
+    for step in range(-1, 2):
+        at = p if step == 0 else torch.nextafter(p, torch.full_like(p, float(step)))
+        _check_sample(x, torch.full((n,), 1.0 - 2.0 ** -24), f"edge {step}", top_p=at.tolist(), min_p=min_p)
+
+
+@pytest.mark.parametrize("temperature", [1e-39, 1e-30, 1e30, 3e38])
+@pytest.mark.parametrize("top_p", [0.7, 1.0])
+def test_sample_extreme_temperatures(temperature, top_p):
+    x = _logits(5, 5003, torch.float32, 81)
+    x[1, :700] = x[1].max() + 1  # ties at the largest value
+    x[2, 40] = math.inf
+    x[3] = torch.finfo(torch.float32).min
+    x[4, ::2] = -math.inf
+    _check_sample(x, torch.rand(5, generator=_gen(82)), "extreme", temperature=temperature, top_p=top_p)
+
+
 def test_sample_settings_per_row():
     n = 24
     g = _gen(9)
