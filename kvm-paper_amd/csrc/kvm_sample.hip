@@ -44,7 +44,8 @@
 // (9 of 16 instructions per logit are the maximum's and the exponential's); 512
 // rows of 65536 bf16 logits with min-p 23 us; one row of 50304 fp32 logits with
 // top-p 16 us where the first list decides (22 with the exact weight of the row
-// on one compute unit), 50 where it does not.
+// on one compute unit), 45 where it does not (the list 13, the histogram 16, the
+// two searches 11 and 8).
 
 #include <type_traits>
 
@@ -253,13 +254,14 @@ __device__ __forceinline__ int collect_above(R &x, const float (&most)[M], uint3
     x.template above<TAKE>(most, least, every, list);
     also(x);
   } else {
-    x.each([&](const float (&v)[N], int i0, int n) {
-      also(v);
+    auto above = [&](const float (&v)[N], bool there) {
+      if (there) also(v);
       float m = v[0];
 #pragma unroll
       for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
-      if ((m >= least || every) && n > 0) list(v, i0, n);
-    });
+      return m >= least || every;
+    };
+    x.where(above, list);
   }
   __syncthreads();
   *hits = {min(sh.hit_chunks, kHitChunks), least, every};
@@ -424,8 +426,20 @@ __device__ __forceinline__ void locate(const R &x, const Weights &wt, u64 target
   uint32_t lo = 0, hi = 0xffffffffu, f_hi = 0, f_span = 0;
   int f_part = -1;
   auto part_of = [&](uint32_t k) { return int(u64(f_hi - k) * kBins / (u64(f_span) + 1)); };
+  // |x - mid| <= half for every value of the bin and few others, whatever the
+  // rounding of either; where that says nothing (an edge is not finite) for all.
+  const float width = 1.f / wt.bins_per;
+  float mid = wt.best - (float(bin) + 0.5f) * width;
+  float half = 0.501f * width + (fabsf(wt.best) + fabsf(mid)) * 0x1p-21f;
+  if (!(half < __builtin_inff())) mid = 0.f, half = __builtin_inff();
   auto tokens = [&](auto &&f) {  // f(key, index, value) for each of them
-    x.template each<1>([&](const float (&v)[N], int i0, int n) {
+    auto near = [&](const float (&v)[N], bool) {
+      bool any = Q == kEvery;
+#pragma unroll
+      for (int i = 0; i < N; ++i) any = any | (fabsf(v[i] - mid) <= half);
+      return any;
+    };
+    x.where(near, [&](const float (&v)[N], int i0, int n) {
       for (uint32_t bits = in_bin<Q, N>(wt, v, n, bin); bits; bits &= bits - 1) {
         const int e = __ffs(bits) - 1, idx = i0 + e;
         float xv = v[0];
@@ -579,6 +593,10 @@ struct Listed {
       f(v, index_of(token), i < cnt ? 1 : 0);
     }
   }
+  template <class W, class F>
+  __device__ __forceinline__ void where(W &&, F &&f) const {
+    each<1>(f);
+  }
 };
 
 // Lists the first tokens of the order, `want` or somewhat more (all that may
@@ -617,7 +635,13 @@ __device__ __forceinline__ int list_first(const R &x, const Weights &wt, int wan
   }
   __syncthreads();
   const float edge = float(sh.bin + 1);
-  x.template each<1>([&](const float (&v)[N], int i0, int n) {
+  auto before = [&](const float (&v)[N], bool) {
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) m = fmaxf(m, v[i]);
+    return wt.place(m) < edge;
+  };
+  x.where(before, [&](const float (&v)[N], int i0, int n) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (wt.place(v[i]) < edge && i < n) {
@@ -1072,7 +1096,8 @@ int64_t top_logits_max() { return kMaxTop; }
 hipError_t launch_sample(const kvm_sample_desc &P, hipStream_t stream) {
   // More rows than compute units: the rows stay in registers.  Fewer: a pass's
   // unrolled code would be read from memory by a workgroup that runs it once
-  // (one row of 50304: 54 us, against 23 with the row read again and loops).
+  // (one row of 50304 when this was measured: 54 us, against 23 with the row read
+  // again in loops).
   const int64_t rows = P.logits.outer * P.logits.inner;
   SampleLaunch l{P, stream};
   if (rows <= 256)
