@@ -33,6 +33,18 @@ void check(int rc, const char *what) {
 
 void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
+// The graph capture that the current stream of t's device is part of (0: none).
+int64_t capture_of(const Tensor &t) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  const auto stream = c10::hip::getCurrentHIPStream(t.device().index()).stream();
+  if (hipStreamGetCaptureInfo(stream, &status, &id) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? int64_t(id) : 0;
+}
+
 int64_t type_code(const Tensor &t, const char *name) {
   switch (t.scalar_type()) {
     case at::kBFloat16: return KVM_BF16;
@@ -228,6 +240,7 @@ class HeadLoss : public torch::autograd::Function<HeadLoss> {
     const Tensor loss = run_loss(logits, a, &grad);
     ctx->save_for_backward({logits, a.labels, a.values, a.indices, a.rest});
     ctx->saved_data["grad"] = grad;
+    ctx->saved_data["capture"] = capture_of(logits);
     ctx->saved_data["temperature"] = a.temperature;
     ctx->saved_data["label_weight"] = a.label_weight;
     ctx->saved_data["ignore_index"] = a.ignore_index;
@@ -246,9 +259,15 @@ class HeadLoss : public torch::autograd::Function<HeadLoss> {
       const at::AutoGradMode no_grad(false);
       const c10::DeviceGuard guard(logits.device());
       auto it = ctx->saved_data.find("grad");
-      if (it != ctx->saved_data.end()) {  // handed out once: what is below may change it
+      if (it != ctx->saved_data.end()) {
         grad = it->second.toTensor();
-        ctx->saved_data.erase(it);
+        // Handed out once, as what is below may change it; a copy of it where
+        // the loss or the gradient is captured without the other, of which one
+        // may run again without the other.
+        if (ctx->saved_data["capture"].toInt() == capture_of(logits))
+          ctx->saved_data.erase(it);
+        else
+          grad = grad.clone();
       } else {  // a retained graph, again
         const LossArgs a{saved[1], saved[2], saved[3], saved[4], ctx->saved_data["temperature"].toDouble(),
                          ctx->saved_data["label_weight"].toDouble(), ctx->saved_data["ignore_index"].toInt(),

@@ -11,6 +11,11 @@ holds a row's logits in registers: a training step moves them once in and
 their gradient once out.  The backward hands that gradient out, multiplied in
 place where the upstream gradient is not one.  Calling backward again on a
 retained graph computes it again.  The losses are differentiable once.
+
+A step may be captured into a HIP graph, with its backward or either alone (the
+backward then hands out a copy).  As for any backward that torch accumulates
+into leaves, no graph of eager steps on the same leaves may be alive while it is
+captured: torch would accumulate on that graph's stream, outside the capture.
 """
 
 from __future__ import annotations

@@ -555,6 +555,50 @@ def test_operators_in_a_captured_graph():
     graph.reset()
 
 
+def test_loss_and_gradient_captured_apart():
+    """A backward replayed on an eager loss gives the same gradient every time,
+    and an eager backward of a replayed loss one that later replays leave alone."""
+    import kvm_amd as K
+
+    x = _logits(17, 1003, torch.float32, 180).to(DEV).requires_grad_(True)
+    labels = torch.randint(0, 1003, (17,), generator=_gen(181)).to(DEV)
+    up = torch.tensor(0.5, device=DEV)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def expected():
+        return torch.autograd.grad(K.cross_entropy(x, labels), x, up)[0]
+
+    with torch.cuda.stream(side):
+        want = expected()
+        loss = K.cross_entropy(x, labels)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        grad, = torch.autograd.grad(loss, x, up, retain_graph=True)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)
+        grad.zero_()
+    graph.reset()
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        loss = K.cross_entropy(x, labels)
+    kept = []
+    for i in range(3):
+        x.data.copy_(_logits(17, 1003, torch.float32, 182 + i))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        kept.append((torch.autograd.grad(loss, x, up, retain_graph=True)[0], expected()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(got, want) for got, want in kept)
+    del loss
+    graph.reset()
+
+
 def test_operators_on_two_streams():
     import kvm_amd as K
 
