@@ -455,7 +455,12 @@ int kvm_sample(const kvm_sample_desc *d, void *stream);
  * same byte offset modulo 16 as the logits' row, for every row) receives
  * d loss / d x.  loss (optional): the sum of row_loss.  inv_count (optional):
  * loss and grad are those of the mean, divided by max(1, rows that count);
- * where there are labels, the word receives the reciprocal of that count. */
+ * where there are labels, the word receives the reciprocal of that count.
+ * upstream (optional, [rows] with upstream_stride 1, or one number with 0):
+ * grad holds the gradient that a call without it wrote; rows whose factor is
+ * not one get it again, times the factor, rounded once (inv_count is then what
+ * that call wrote, row_loss is written for those rows only, and loss may not be
+ * asked for). */
 typedef struct kvm_head_loss_desc {
   kvm_logits logits;
   const int64_t *labels;    /* [rows] or NULL (needs a teacher) */
@@ -472,6 +477,8 @@ typedef struct kvm_head_loss_desc {
   float *loss;              /* out [1] or NULL */
   void *grad;               /* out or NULL */
   int64_t g_outer, g_inner;
+  const float *upstream;
+  int64_t upstream_stride;
 } kvm_head_loss_desc;
 
 int kvm_head_loss(const kvm_head_loss_desc *d, void *stream);
@@ -479,7 +486,7 @@ int kvm_head_loss(const kvm_head_loss_desc *d, void *stream);
 /* rows->data (written in place) times factor[r * factor_stride] of its row r
  * (stride 0: one factor for all), products in fp32, rounded once; rows whose
  * factor is 1 are not touched.  The backward of kvm_head_loss for an upstream
- * gradient other than one. */
+ * gradient other than one, but for fp16 (upstream there). */
 int kvm_scale_rows(const kvm_logits *rows, const float *factor, int64_t factor_stride, void *stream);
 
 /* ABI self-description, checked by the host binding at load time. */

@@ -305,6 +305,8 @@ int kvm_head_loss(const kvm_head_loss_desc *d, void *stream) {
       return fail(KVM_EINVAL, "head_loss: label_weight must be in [0, 1]");
     if (P.label_weight > 0.0 && !P.labels) return fail(KVM_EINVAL, "head_loss: label_weight needs labels");
   }
+  if (P.upstream && (!P.grad || P.loss || P.upstream_stride < 0))
+    return fail(KVM_EINVAL, "head_loss: upstream needs grad, a stride >= 0, and no loss");
   if (P.grad) {
     if (P.grad == P.logits.data) return fail(KVM_EINVAL, "head_loss: grad may not be the logits");
     // Same offset modulo 16 bytes in every row: the gradient is stored in the chunks the logits are read in.

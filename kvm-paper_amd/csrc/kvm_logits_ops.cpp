@@ -180,7 +180,8 @@ struct LossArgs {
 // A tensor shaped as the logits whose rows start at the same offset modulo 16
 // bytes as the logits' rows (the kernel stores it in the chunks it loads), with
 // as little padding between them as that takes.
-Tensor gradient_like(const Tensor &logits, const kvm_logits &L, int64_t *g_outer, int64_t *g_inner) {
+Tensor gradient_like(const Tensor &logits, const kvm_logits &L, int64_t *g_outer, int64_t *g_inner,
+                     bool strides_only = false) {
   const int64_t size = logits.element_size(), n = 16 / size;
   auto mod = [n](int64_t v) { return ((v % n) + n) % n; };
   const int64_t gi = L.inner > 1 ? L.vocab + mod(L.s_inner - L.vocab) : L.vocab;
@@ -188,13 +189,19 @@ Tensor gradient_like(const Tensor &logits, const kvm_logits &L, int64_t *g_outer
   const int64_t offset = int64_t(reinterpret_cast<uintptr_t>(L.data) % 16) / size;
   *g_outer = go;
   *g_inner = gi;
+  if (strides_only) return {};
   if (gi == L.vocab && go == L.inner * gi && offset == 0) return at::empty(logits.sizes(), logits.options());
   return at::empty({offset + L.outer * go}, logits.options())
       .as_strided({L.outer, L.inner, L.vocab}, {go, gi, 1}, offset)
       .view(logits.sizes());
 }
 
-Tensor run_loss(const Tensor &logits, const LossArgs &a, Tensor *grad) {
+// The loss, and with grad its gradient for an upstream gradient of one;
+// *row_losses receives the losses of the rows, and behind them the scratch of
+// a mean.  With upstream, *grad and *row_losses are those of such a call, and
+// the gradient is made again times upstream; the result is then nothing.
+Tensor run_loss(const Tensor &logits, const LossArgs &a, Tensor *grad, Tensor *row_losses,
+                const Tensor &upstream = {}) {
   const c10::DeviceGuard guard(logits.device());
   Tensor held;
   kvm_head_loss_desc d{};
@@ -213,19 +220,25 @@ Tensor run_loss(const Tensor &logits, const LossArgs &a, Tensor *grad) {
   d.temperature = a.temperature;
   const auto f32 = logits.options().dtype(at::kFloat);
   Tensor loss;
-  // The row losses, and behind them the scratch of a mean.
-  const Tensor per_row = a.reduction == kNone ? at::empty(rows_shape(logits), f32) : at::empty({rows + 1}, f32);
+  Tensor &per_row = *row_losses;
+  if (!upstream.defined() || a.reduction == kNone)  // the losses a caller got are left as they are
+    per_row = a.reduction == kNone ? at::empty(rows_shape(logits), f32) : at::empty({rows + 1}, f32);
   d.row_loss = per_row.data_ptr<float>();
   if (a.reduction != kNone) {
-    loss = at::empty({}, f32);
-    d.loss = loss.data_ptr<float>();
+    if (!upstream.defined()) {
+      loss = at::empty({}, f32);
+      d.loss = loss.data_ptr<float>();
+    }
     if (a.reduction == kMean) d.inv_count = d.row_loss + rows;
   } else {
     loss = per_row;
   }
   if (grad) {
-    *grad = gradient_like(logits, d.logits, &d.g_outer, &d.g_inner);
+    const Tensor fresh = gradient_like(logits, d.logits, &d.g_outer, &d.g_inner, upstream.defined());
+    if (fresh.defined()) *grad = fresh;
     d.grad = grad->data_ptr();
+    d.upstream = data_of<float>(upstream);
+    d.upstream_stride = upstream.defined() && upstream.dim() ? 1 : 0;
   }
   check(kvm_head_loss(&d, stream_of(logits)), "head_loss");
   return loss;
@@ -236,10 +249,11 @@ class HeadLoss : public torch::autograd::Function<HeadLoss> {
   // The gradient for an upstream gradient of one is made with the loss, while
   // a row is in registers, and kept for the backward.
   static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &logits, const LossArgs &a) {
-    Tensor grad;
-    const Tensor loss = run_loss(logits, a, &grad);
+    Tensor grad, rows;
+    const Tensor loss = run_loss(logits, a, &grad, &rows);
     ctx->save_for_backward({logits, a.labels, a.values, a.indices, a.rest});
     ctx->saved_data["grad"] = grad;
+    if (a.reduction != kNone && logits.scalar_type() == at::kHalf) ctx->saved_data["rows"] = rows;
     ctx->saved_data["capture"] = capture_of(logits);
     ctx->saved_data["temperature"] = a.temperature;
     ctx->saved_data["label_weight"] = a.label_weight;
@@ -258,26 +272,36 @@ class HeadLoss : public torch::autograd::Function<HeadLoss> {
     {
       const at::AutoGradMode no_grad(false);
       const c10::DeviceGuard guard(logits.device());
+      const LossArgs a{saved[1], saved[2], saved[3], saved[4], ctx->saved_data["temperature"].toDouble(),
+                       ctx->saved_data["label_weight"].toDouble(), ctx->saved_data["ignore_index"].toInt(),
+                       ctx->saved_data["reduction"].toInt()};
       auto it = ctx->saved_data.find("grad");
-      if (it != ctx->saved_data.end()) {
-        grad = it->second.toTensor();
-        // Handed out once, as what is below may change it; a copy of it where
-        // the loss or the gradient is captured without the other, of which one
-        // may run again without the other.
-        if (ctx->saved_data["capture"].toInt() == capture_of(logits))
-          ctx->saved_data.erase(it);
-        else
-          grad = grad.clone();
-      } else {  // a retained graph, again
-        const LossArgs a{saved[1], saved[2], saved[3], saved[4], ctx->saved_data["temperature"].toDouble(),
-                         ctx->saved_data["label_weight"].toDouble(), ctx->saved_data["ignore_index"].toInt(),
-                         ctx->saved_data["reduction"].toInt()};
-        run_loss(logits, a, &grad);
+      Tensor rows;
+      if (auto kept = ctx->saved_data.find("rows"); kept != ctx->saved_data.end()) rows = kept->second.toTensor();
+      if (it == ctx->saved_data.end()) {  // a retained graph, again
+        run_loss(logits, a, &grad, &rows);
+      } else if (ctx->saved_data["capture"].toInt() == capture_of(logits)) {
+        grad = it->second.toTensor();  // handed out once, as what is below may change it
+        ctx->saved_data.erase(it);
+      } else {
+        // A copy where the loss or the gradient is captured without the other,
+        // of which one may run again without the other.
+        int64_t outer, inner;
+        Tensor held;
+        grad = gradient_like(logits, rows_of(logits, "logits", &held), &outer, &inner);
+        grad.copy_(it->second.toTensor());
       }
       const Tensor up = ups[0].to(at::kFloat).contiguous();
-      Tensor held;
-      const kvm_logits L = rows_of(grad, "gradient", &held);
-      check(kvm_scale_rows(&L, up.data_ptr<float>(), up.dim() ? 1 : 0, stream_of(grad)), "head_loss backward");
+      if (grad.scalar_type() == at::kHalf) {
+        // fp16 ends at 2^-24, where the gradient of a mean over a batch often
+        // lies, and a loss scaled against that has its factor here: the gradient
+        // is made again, rounded with the factor in it.  The traffic is the same.
+        run_loss(logits, a, &grad, &rows, up);
+      } else {
+        Tensor held;
+        const kvm_logits L = rows_of(grad, "gradient", &held);
+        check(kvm_scale_rows(&L, up.data_ptr<float>(), up.dim() ? 1 : 0, stream_of(grad)), "head_loss backward");
+      }
     }
     if (at::GradMode::is_enabled()) {
       auto twice = std::make_shared<torch::autograd::DelayedError>(
@@ -330,7 +354,8 @@ Tensor head_loss(const Tensor &logits, const OptTensor &labels, const OptTensor 
   if (differentiable)
     return HeadLoss::apply(held, a);
   const at::AutoGradMode no_grad(false);
-  return run_loss(held, a, nullptr);
+  Tensor rows;
+  return run_loss(held, a, nullptr, &rows);
 }
 
 }  // namespace

@@ -100,6 +100,9 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
     const int o = row / int(P.logits.inner), i = row - o * int(P.logits.inner);
     grad = static_cast<raw *>(P.grad) + o * P.g_outer + i * P.g_inner;
   }
+  // A gradient made again for an upstream gradient: rows for which it is one have theirs.
+  const float up = P.upstream ? P.upstream[row * P.upstream_stride] : 1.f;
+  if (P.upstream && up == 1.f) return;
   int64_t label = P.labels ? P.labels[row] : 0;
   const bool ignored = P.labels && label == P.ignore_index;
   // The teacher's first entries are asked for before the row: what depends on
@@ -127,7 +130,7 @@ __global__ __launch_bounds__(T) __attribute__((amdgpu_waves_per_eu(4))) void k_h
     return;
   }
   const float a = P.labels ? float(P.label_weight) : 0.f;  // weight of the hard labels
-  float scale = P.inv_count && P.labels ? *P.inv_count : every_row;
+  float scale = (P.inv_count && P.labels ? *P.inv_count : every_row) * up;
   // A label outside the vocabulary (and not ignored) makes the row's loss and gradient NaN.
   const bool bad = P.labels && (label < 0 || label >= V);
   if (bad) {
@@ -508,7 +511,7 @@ hipError_t launch_head_loss(const kvm_head_loss_desc &P, hipStream_t stream) {
   // A mean's factor: counted from the labels, or known.
   const float *counted = P.labels ? P.inv_count : nullptr;
   const float every_row = P.inv_count && !P.labels ? 1.f / float(rows) : 1.f;
-  if (counted)
+  if (counted && !P.upstream)
     hipLaunchKernelGGL(k_count_labels, dim3(1), dim3(1024), 0, stream, P.labels, rows, P.ignore_index, P.inv_count);
   LossLaunch l{P, every_row, stream};
   with_row<true>(P.logits.vocab, P.logits.dtype, 256, l);

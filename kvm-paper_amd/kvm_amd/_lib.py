@@ -176,6 +176,7 @@ class KvmHeadLossDesc(ctypes.Structure):
         ("temperature", ctypes.c_double),
         ("row_loss", _vp), ("inv_count", _vp), ("loss", _vp),
         ("grad", _vp), ("g_outer", _i64), ("g_inner", _i64),
+        ("upstream", _vp), ("upstream_stride", _i64),
     ]
 
 

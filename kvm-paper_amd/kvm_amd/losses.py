@@ -9,7 +9,9 @@ the logits' type.
 The forward computes the gradient for an upstream gradient of one while it
 holds a row's logits in registers: a training step moves them once in and
 their gradient once out.  The backward hands that gradient out, multiplied in
-place where the upstream gradient is not one.  Calling backward again on a
+place where the upstream gradient is not one; in float16, whose small numbers
+end at 2^-24, it is computed again with the factor in it, so that a scaled loss
+keeps what the scale is for.  Calling backward again on a
 retained graph computes it again.  The losses are differentiable once.
 
 A step may be captured into a HIP graph, with its backward or either alone (the

@@ -480,6 +480,35 @@ def test_loss_upstream_gradients_and_retained_graphs():
     empty.backward()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("rows,V", [((2, 300), 5003), ((3, 7), 999)])
+def test_scaled_losses_keep_small_gradients(dtype, reduction, rows, V):
+    """A loss times 2^14 whose unscaled gradient is below fp16's smallest number."""
+    import kvm_amd as K
+
+    n = rows[0] * rows[1]
+    wide = _logits(n, V + 5, dtype, 115, 1.0).view(*rows, V + 5)
+    labels = torch.randint(0, V, rows, generator=_gen(116))
+    labels[0, 3] = -100
+    x = wide.to(DEV).requires_grad_(True)
+    loss = K.cross_entropy(x[..., 2:V + 2], labels.to(DEV), reduction=reduction)
+    up = torch.full(loss.shape, 2.0 ** 14, device=DEV)
+    if reduction == "none":
+        up[0, :2] = 1.0
+    for retain in (True, False):
+        got = torch.autograd.grad(loss, x, up, retain_graph=retain)[0][..., 2:V + 2].double().cpu()
+        p = torch.softmax(wide[..., 2:V + 2].double(), -1)
+        hot = torch.zeros_like(p).scatter_(-1, labels.clamp(min=0)[..., None], 1.0)
+        f = (up.double().cpu().expand(rows) / (n - 1 if reduction == "mean" else 1) * (labels != -100))[..., None]
+        want, size = (p - hot) * f, (p + hot) * f
+        # one rounding of the result (two where the kept gradient is scaled, and the smallest numbers of both)
+        roundings = 1 if dtype == torch.float16 else 2
+        tiny = TINY[dtype] * (1 if dtype == torch.float16 else 2.0 ** 14 + 1)
+        bar = roundings * torch.finfo(dtype).eps / 2 * want.abs() + 3 * SUM * size + tiny
+        assert bool(((got - want).abs() <= bar).all())
+
+
 def test_loss_is_the_same_every_time():
     import kvm_amd as K
 
